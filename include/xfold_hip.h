@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define XFH_ABI_VERSION 11
+#define XFH_ABI_VERSION 12
 
 enum { XFH_F32 = 0, XFH_BF16 = 1, XFH_BOOL = 2 };
 enum { XFH_OK = 0, XFH_EINVAL = 1, XFH_EUNSUPPORTED = 2, XFH_EWORKSPACE = 3, XFH_EHIP = 4 };
@@ -437,6 +437,59 @@ int xfh_cross_attention_bias(const void *pair_logits, int logits_dtype, const in
  * (xfold/fastnn/native.py:31-43 computes in the autocast dtype); the hip modules run it here
  * instead of in a torch kernel. */
 int xfh_convert(const void *x, int x_dtype, void *y, int y_dtype, int64_t n, void *stream);
+
+/* LayerNorm for training, over the last dim of [rows, cols] (x row stride ldx, y contiguous), and its
+ * backward pass. x and y: f32 and f32, bf16 and bf16, or bf16 and f32. weight and bias in types of
+ * their own (NULL = absent). stats (fp32 [rows][2]: mean, 1 / sqrt(variance + eps); NULL in a forward
+ * pass that needs no backward one) goes from one to the other. dy is in y's type (row stride lddy),
+ * dx in x's (contiguous); dx, dweight and dbias may each be NULL. No rows: dweight and dbias are
+ * zeros. Sums are taken in a fixed order: a call gives the same bits every time. Beside the
+ * LayerNorm backends of xfold/fastnn/layer_norm.py:55-81, which serve inference. (ABI 12.) */
+int xfh_layer_norm_train(const void *x, int x_dtype, int64_t ldx, int64_t rows, int64_t cols, const void *weight,
+                         int weight_dtype, const void *bias, int bias_dtype, float eps, void *y, int y_dtype,
+                         float *stats, void *stream);
+int64_t xfh_layer_norm_backward_workspace_size(int64_t rows, int64_t cols);
+int xfh_layer_norm_backward(const void *dy, int dy_dtype, int64_t lddy, const void *x, int x_dtype, int64_t ldx,
+                            int64_t rows, int64_t cols, const void *weight, int weight_dtype, const float *stats,
+                            void *dx, void *dweight, int dweight_dtype, void *dbias, int dbias_dtype,
+                            void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Arguments of the sequence attention (host struct; strides in elements, the last dims contiguous). */
+typedef struct XfhSequenceAttention {
+  const void *q, *k, *v;           /* [batch][heads][queries][dim], [batch][kv_heads][keys][dim], [..][keys][value_dim] */
+  void *out;                       /* [batch][heads][queries][value_dim]; read by the backward pass */
+  float *lse;                      /* fp32 [batch][heads][queries], for the backward pass; NULL: none */
+  const float *slopes;             /* fp32 [heads], or NULL */
+  const int32_t *prefix;           /* [batch], or NULL: prefix_all for every entry */
+  const int32_t *documents;        /* [batch][keys] (row stride documents_stride), or NULL */
+  const int32_t *lengths;          /* [batch], or NULL: every entry has `keys` keys */
+  const void *dout;                /* backward: as out */
+  void *dq, *dk, *dv;              /* backward: as q, k, v */
+  float *dslopes;                  /* backward: fp32 [heads], or NULL */
+  int64_t batch, heads, kv_heads, queries, keys, dim, value_dim;
+  int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3];
+  int64_t dout_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
+  int64_t documents_stride, prefix_all;
+  float scale, softcap;            /* softcap <= 0: no cap */
+  int causal, dtype;
+} XfhSequenceAttention;
+
+/* Attention over token sequences, forward and backward; bf16 or f32, dim and value_dim 1 to 128,
+ * heads a multiple of kv_heads (head h reads key head h / (heads / kv_heads)).
+ *   score(i, j) = c(scale q_i . k_j) - slopes[h] |p_i - j|,  c(x) = softcap tanh(x / softcap)
+ * The queries are the last ones of a sequence of n = lengths[b] tokens (or `keys`): p_i = n - queries + i.
+ * Query i sees key j iff j < n, and (not causal, or j <= p_i, or j < prefix), and documents[p_i] ==
+ * documents[j] >= 0; with lengths, a query with p_i < 0 sees nothing. A query that sees no key gives
+ * zeros, and takes and gives no gradient. A place that is masked does not matter, whatever it holds
+ * (NaN and infinities too), and keys from n on are not read; their dk and dv are zeros. lengths
+ * are held to [0, keys]. queries > keys is for calls without causal, documents and lengths.
+ * The backward pass takes what the forward pass got and gave. Its sums have a fixed order: the
+ * same bits every time. Beside dot_product_attention (xfold/fastnn/attention.py:45-98), which has
+ * additive biases and key masks, and no gradient. (ABI 12.) */
+int64_t xfh_sequence_attention_workspace_size(const XfhSequenceAttention *args);
+int xfh_sequence_attention(const XfhSequenceAttention *args, void *workspace, int64_t workspace_bytes, void *stream);
+int64_t xfh_sequence_attention_backward_workspace_size(const XfhSequenceAttention *args);
+int xfh_sequence_attention_backward(const XfhSequenceAttention *args, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -898,4 +898,138 @@ int xfh_pairformer_single(void *pair, void *single, int single_dtype, int64_t n,
                         w.w2, XFH_BF16, single, single_dtype, 1, transition_ws, rest, stream);
 }
 
+int xfh_layer_norm_train(const void *x, int x_dtype, int64_t ldx, int64_t rows, int64_t cols, const void *weight,
+                         int weight_dtype, const void *bias, int bias_dtype, float eps, void *y, int y_dtype,
+                         float *stats, void *stream) {
+  XFH_REQUIRE(rows >= 0 && cols >= 0 && cols <= (int64_t(1) << 30), "layer_norm_train: bad size");
+  XFH_REQUIRE(float_dtype(x_dtype) && float_dtype(y_dtype) && (!weight || float_dtype(weight_dtype)) &&
+                  (!bias || float_dtype(bias_dtype)), "layer_norm_train: dtypes must be f32/bf16");
+  XFH_REQUIRE(eps >= 0.f, "layer_norm_train: eps must be nonnegative");
+  XFH_REQUIRE(rows == 0 || cols == 0 || (x && y), "layer_norm_train: null tensor");
+  XFH_REQUIRE(rows <= 1 || ldx >= cols, "layer_norm_train: row stride too small");
+  return norm_train_forward(x, x_dtype, ldx, rows, cols, weight, weight_dtype, bias, bias_dtype, eps, y, y_dtype, stats,
+                            as_stream(stream));
+}
+
+int64_t xfh_layer_norm_backward_workspace_size(int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 0 || cols > (int64_t(1) << 30)) return -1;
+  return norm_train_backward_workspace(rows, cols);
+}
+
+int xfh_layer_norm_backward(const void *dy, int dy_dtype, int64_t lddy, const void *x, int x_dtype, int64_t ldx,
+                            int64_t rows, int64_t cols, const void *weight, int weight_dtype, const float *stats,
+                            void *dx, void *dweight, int dweight_dtype, void *dbias, int dbias_dtype,
+                            void *workspace, int64_t workspace_bytes, void *stream) {
+  XFH_REQUIRE(rows >= 0 && cols >= 0 && cols <= (int64_t(1) << 30), "layer_norm_backward: bad size");
+  XFH_REQUIRE(float_dtype(x_dtype) && float_dtype(dy_dtype) && (!weight || float_dtype(weight_dtype)) &&
+                  (!dweight || float_dtype(dweight_dtype)) && (!dbias || float_dtype(dbias_dtype)),
+              "layer_norm_backward: dtypes must be f32/bf16");
+  XFH_REQUIRE(rows == 0 || cols == 0 || (x && dy && stats), "layer_norm_backward: null tensor");
+  XFH_REQUIRE(rows <= 1 || (ldx >= cols && lddy >= cols), "layer_norm_backward: row stride too small");
+  if (dweight || dbias) {
+    const int64_t need = norm_train_backward_workspace(rows, cols);
+    if (need > 0 && (!workspace || need > workspace_bytes))
+      return fail(XFH_EWORKSPACE, "layer_norm_backward: workspace too small (need " + std::to_string(need) + " bytes)");
+  }
+  return norm_train_backward(dy, dy_dtype, lddy, x, x_dtype, ldx, rows, cols, weight, weight_dtype, stats, dx, dweight,
+                             dweight_dtype, dbias, dbias_dtype, static_cast<float *>(workspace), as_stream(stream));
+}
+
+}  // extern "C"
+
+namespace xfh {
+
+// Checks of both directions; fills the kernels' arguments.
+static int sequence_args(const XfhSequenceAttention *p, SequenceArgs &a) {
+  XFH_REQUIRE(p, "sequence_attention: null argument");
+  XFH_REQUIRE(float_dtype(p->dtype), "sequence_attention: dtype must be f32/bf16");
+  const int64_t most = (int64_t(1) << 31) - 129;
+  for (int64_t n : {p->batch, p->heads, p->kv_heads, p->queries, p->keys})
+    XFH_REQUIRE(n >= 0 && n <= most, "sequence_attention: sizes must fit in 31 bits");
+  XFH_REQUIRE(p->dim > 0 && p->dim <= 128 && p->value_dim > 0 && p->value_dim <= 128,
+              "sequence_attention: head dims must be 1 to 128");
+  XFH_REQUIRE(p->heads == 0 || (p->kv_heads > 0 && p->heads % p->kv_heads == 0),
+              "sequence_attention: heads must be a multiple of the key heads");
+  XFH_REQUIRE(p->queries <= p->keys || !(p->causal || p->documents || p->lengths),
+              "sequence_attention: more queries than keys with a causal, document or length mask");
+  XFH_REQUIRE(p->causal || !(p->prefix || p->prefix_all), "sequence_attention: a prefix needs the causal mask");
+  XFH_REQUIRE(std::isfinite(p->scale) && std::isfinite(p->softcap), "sequence_attention: scale and softcap must be finite");
+  std::memset(&a, 0, sizeof(a));
+  a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.lse = p->lse; a.slopes = p->slopes;
+  a.prefix = p->prefix; a.documents = p->documents; a.lengths = p->lengths;
+  a.dout = p->dout; a.dq = p->dq; a.dk = p->dk; a.dv = p->dv;
+  a.documents_stride = p->documents_stride;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = p->q_strides[i]; a.ks[i] = p->k_strides[i]; a.vs[i] = p->v_strides[i]; a.os[i] = p->out_strides[i];
+    a.gs[i] = p->dout_strides[i]; a.dqs[i] = p->dq_strides[i]; a.dks[i] = p->dk_strides[i]; a.dvs[i] = p->dv_strides[i];
+  }
+  a.B = int(p->batch); a.H = int(p->heads); a.Hk = int(p->kv_heads); a.Nq = int(p->queries); a.Nk = int(p->keys);
+  a.D = int(p->dim); a.Dv = int(p->value_dim);
+  a.tiles = int(ceil_div(p->keys, int64_t(64)));
+  a.scale = p->scale;
+  a.cap = p->softcap > 0.f ? p->softcap : 0.f;
+  a.causal = p->causal != 0;
+  a.prefix_all = int(std::min(std::max(p->prefix_all, int64_t(0)), p->keys));
+  return XFH_OK;
+}
+
+struct SequencePlan { void *ranges; float *delta, *slope_part; };
+static int64_t sequence_carve(Carver &cv, SequencePlan &p, const SequenceArgs &a, bool backward, bool slopes) {
+  std::memset(&p, 0, sizeof(p));
+  if (a.documents) p.ranges = cv.take(sequence_ranges_bytes(a.B, a.Nk));
+  if (backward) {
+    p.delta = static_cast<float *>(cv.take(int64_t(a.B) * a.H * a.Nq * 4));
+    if (slopes) p.slope_part = static_cast<float *>(cv.take(sequence_slope_part(a.B, a.H, a.Nq) * 4));
+  }
+  return cv.used;
+}
+
+}  // namespace xfh
+
+extern "C" {
+
+int64_t xfh_sequence_attention_workspace_size(const XfhSequenceAttention *args) {
+  SequenceArgs a;
+  SequencePlan p;
+  Carver cv(nullptr, 0);
+  return sequence_args(args, a) == XFH_OK ? sequence_carve(cv, p, a, false, false) : -1;
+}
+
+int xfh_sequence_attention(const XfhSequenceAttention *args, void *workspace, int64_t workspace_bytes, void *stream) {
+  SequenceArgs a;
+  SequencePlan p;
+  XFH_TRY(sequence_args(args, a));
+  if (a.B == 0 || a.H == 0 || a.Nq == 0) return XFH_OK;
+  XFH_REQUIRE(a.q && a.out && (a.Nk == 0 || (a.k && a.v)), "sequence_attention: null tensor");
+  Carver cv(workspace, workspace_bytes);
+  if (sequence_carve(cv, p, a, false, false) > (workspace ? workspace_bytes : 0))
+    return fail(XFH_EWORKSPACE, "sequence_attention: workspace too small (need " + std::to_string(cv.used) + " bytes)");
+  a.ranges = p.ranges;
+  return sequence_forward(a, args->dtype, as_stream(stream));
+}
+
+int64_t xfh_sequence_attention_backward_workspace_size(const XfhSequenceAttention *args) {
+  SequenceArgs a;
+  SequencePlan p;
+  Carver cv(nullptr, 0);
+  return sequence_args(args, a) == XFH_OK ? sequence_carve(cv, p, a, true, args->dslopes != nullptr) : -1;
+}
+
+int xfh_sequence_attention_backward(const XfhSequenceAttention *args, void *workspace, int64_t workspace_bytes, void *stream) {
+  SequenceArgs a;
+  SequencePlan p;
+  XFH_TRY(sequence_args(args, a));
+  XFH_REQUIRE(!args->dslopes || a.slopes, "sequence_attention_backward: no slopes to take a gradient of");
+  const bool queries = a.B > 0 && a.H > 0 && a.Nq > 0, keys = a.B > 0 && a.Hk > 0 && a.Nk > 0;
+  XFH_REQUIRE(!queries || (a.q && a.out && a.lse && a.dout && a.dq), "sequence_attention_backward: null tensor");
+  XFH_REQUIRE(!keys || (a.k && a.v && a.dk && a.dv), "sequence_attention_backward: null tensor");
+  Carver cv(workspace, workspace_bytes);
+  if (sequence_carve(cv, p, a, true, args->dslopes != nullptr) > (workspace ? workspace_bytes : 0))
+    return fail(XFH_EWORKSPACE, "sequence_attention_backward: workspace too small (need " + std::to_string(cv.used) + " bytes)");
+  a.ranges = p.ranges;
+  a.delta = p.delta;
+  a.slope_part = p.slope_part;
+  return sequence_backward(a, args->dtype, args->dslopes, as_stream(stream));
+}
+
 }  // extern "C"

@@ -289,4 +289,36 @@ int msa_output(const MsaOutputArgs &a, int x_dtype, int out_dtype, hipStream_t s
 int trimul_gate(const void *proj, const void *gate, int dtype, const void *mask, int mask_dtype,
                 int64_t n, int64_t c, int outgoing, void *a_out, void *b_out, hipStream_t s);
 
+// LayerNorm with its statistics kept (stats [rows][2] = mean, 1 / deviation, or null) and its backward
+// pass (norm_train.hip). partial: norm_train_backward_workspace bytes, used when dw or db is given.
+int norm_train_forward(const void *x, int x_dtype, int64_t ldx, int64_t rows, int64_t cols, const void *w, int w_dtype,
+                       const void *b, int b_dtype, float eps, void *y, int y_dtype, float *stats, hipStream_t s);
+int64_t norm_train_backward_workspace(int64_t rows, int64_t cols);
+int norm_train_backward(const void *dy, int dy_dtype, int64_t lddy, const void *x, int x_dtype, int64_t ldx, int64_t rows,
+                        int64_t cols, const void *w, int w_dtype, const float *stats, void *dx, void *dw, int dw_dtype,
+                        void *db, int db_dtype, float *partial, hipStream_t s);
+
+// Sequence attention (sequence.h): q, out, dout, dq [B][H][Nq][.], k, v, dk, dv [B][Hk][Nk][.], strides of
+// the first three dims in elements, the last dim contiguous.
+struct SequenceArgs {
+  const void *q, *k, *v, *dout;
+  void *out, *dq, *dk, *dv;
+  float *lse;                // [B][H][Nq], log2 of the sum of exp2 of the scores; +inf: no visible key
+  float *delta;              // [B][H][Nq], dout . out
+  float *slope_part;         // [H][B][query tiles], or null
+  const float *slopes;       // [H], or null
+  const int32_t *prefix, *documents, *lengths;
+  const void *ranges;        // [B][tiles] seq::Range, with documents
+  int64_t documents_stride;
+  int64_t qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];
+  int B, H, Hk, Nq, Nk, D, Dv, tiles;
+  float scale, cap;
+  int causal, prefix_all;
+};
+int64_t sequence_ranges_bytes(int64_t B, int64_t Nk);
+int sequence_ranges(const SequenceArgs &a, hipStream_t s);
+int sequence_forward(const SequenceArgs &a, int dtype, hipStream_t s);
+int64_t sequence_slope_part(int64_t B, int64_t H, int64_t Nq);   // floats
+int sequence_backward(const SequenceArgs &a, int dtype, float *dslopes, hipStream_t s);
+
 }  // namespace xfh

@@ -1,0 +1,79 @@
+// Sequence attention: what its kernels share (arguments, masks, scores).
+//
+//   x_ij = scale q_i . k_j,  c_ij = cap tanh(x_ij / cap) (cap > 0),  s_ij = c_ij - slope_h |p_i - j|
+//   O_i = sum_j P_ij v_j,  P_ij = exp(s_ij - L_i) over the visible keys,  L_i = log sum exp s_ij
+// p_i = i + n - Nq is the place of query i in its sequence of n tokens. Query i sees key j iff
+//   j < n, and (not causal, or j <= p_i, or j < prefix), and document[p_i] == document[j] >= 0.
+// For one query all but the documents is one bound, j < limit; 0 where it sees nothing.
+// Scores and L are held in units of log 2 (the kernels take exp2).
+#pragma once
+
+#include "common.h"
+#include "kernels.h"
+
+namespace xfh {
+namespace seq {
+
+constexpr int kTile = 64;                  // tokens of a tile: keys of a loop step, and document ranges
+
+// Documents of a tile of 64 keys: the lowest and highest of its kept keys (lo > hi: none), and
+// whether all 64 are kept.
+typedef int4 Range;                        // lo, hi, full, unused
+
+struct Place { int n, prefix, shift; };    // of one batch entry: tokens, prefix, p_i - i
+
+__device__ __forceinline__ Place place_of(const SequenceArgs &a, int b) {
+  Place p;
+  p.n = a.lengths ? min(max(a.lengths[b], 0), a.Nk) : a.Nk;
+  p.prefix = a.prefix ? a.prefix[b] : a.prefix_all;
+  p.shift = p.n - a.Nq;
+  return p;
+}
+// Bound on the keys of query i < Nq, documents aside. It does not fall as i rises.
+__device__ __forceinline__ int limit_of(const SequenceArgs &a, const Place &p, int i) {
+  const int pos = i + p.shift;
+  if (a.lengths && pos < 0) return 0;
+  return a.causal ? min(p.n, max(pos + 1, p.prefix)) : p.n;
+}
+struct Row { int limit, document, pos; };
+__device__ __forceinline__ Row row_of(const SequenceArgs &a, const Place &p, int b, int i) {
+  Row r{0, 0, i + p.shift};
+  if (i >= a.Nq) return r;
+  r.limit = limit_of(a, p, i);
+  if (a.documents) {
+    r.document = r.pos >= 0 && r.pos < p.n ? a.documents[int64_t(b) * a.documents_stride + r.pos] : -1;
+    if (r.document < 0) r.limit = 0;
+  }
+  return r;
+}
+
+// Range of the documents of queries [i0, i1] (at most 64 of them: they lie in two tiles).
+__device__ __forceinline__ Range query_range(const SequenceArgs &a, const Place &p, int b, int i0, int i1) {
+  const int p0 = max(i0 + p.shift, 0), p1 = i1 + p.shift;
+  if (p1 < 0) return Range{0x7fffffff, -1, 0, 0};
+  const Range *r = static_cast<const Range *>(a.ranges) + int64_t(b) * a.tiles;
+  Range u = r[p0 / kTile];
+  const Range w = r[p1 / kTile];
+  u.x = min(u.x, w.x);
+  u.y = max(u.y, w.y);
+  u.z = u.z & w.z;
+  return u;
+}
+__device__ __forceinline__ bool overlap(const Range &u, const Range &w) { return u.x <= w.y && w.x <= u.y; }
+// Every pair of a token of one and a token of the other is in one document.
+__device__ __forceinline__ bool same_document(const Range &u, const Range &w) {
+  return u.z && w.z && u.x == u.y && w.x == w.y && u.x == w.x;
+}
+
+// c / cap and its slope. fp32: the library's tanh. bf16: 1 - 2 / (exp(2 t) + 1) on the hardware's
+// exp2 and reciprocal, off by at most about 2^-22 (a score of 50 by 1e-5, far below the step of P in bf16).
+template <typename T> __device__ __forceinline__ float bend(float t);
+template <> __device__ __forceinline__ float bend<float>(float t) { return tanhf(t); }
+template <> __device__ __forceinline__ float bend<bf16>(float t) {
+  const float e = __builtin_amdgcn_exp2f(t * (2.0f * kLog2e));
+  return 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+}
+template <typename T> __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+}  // namespace seq
+}  // namespace xfh

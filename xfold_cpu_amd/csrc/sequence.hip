@@ -1,0 +1,600 @@
+// Sequence attention for any head dim up to 128 in bf16 and fp32: forward, dq, dk and dv.
+//
+// A workgroup owns 64 tokens (16 per wavefront, one per lane column): queries in the forward pass and
+// for dq, keys for dk and dv. It walks the other side in tiles of 64, held row-major in LDS. With the
+// owned tokens as the columns of every product,
+//   forward  S^T = K Q^T                     O^T  += V^T P^T
+//   dq       S^T = K Q^T, dP^T = V dO^T      dQ^T += K^T dS^T
+//   dk, dv   S = Q K^T, dP = dO V^T          dV^T += dO^T P, dK^T += Q^T dS
+// a lane holds four rows of one column after the first products, which is the B operand of the
+// second ones up to a permutation of the 32 rows of a step; the A operand read applies the same. So no
+// score leaves its lane but for the sums over the four lanes of a column.
+//
+// Tiles that no owned token sees are skipped: a wavefront tests 64 tiles at a time, one per lane.
+//
+// What a masked place holds does not matter: its score is replaced and its weight is 0, but in the
+// second products 0 times an infinity or a NaN of the other side is NaN. Such a sum cannot become
+// finite again, so one test of the results finds it, and the tile loop runs once more in a form that
+// takes these elements out of the operand (as 0) and adds them to the rows that see them.
+#include <algorithm>
+#include <initializer_list>
+#include <utility>
+
+#include "sequence.h"
+
+namespace xfh {
+namespace {
+
+using namespace seq;
+
+// Range of each tile of 64 keys: one wavefront per tile.
+__global__ __launch_bounds__(256) void ranges_kernel(SequenceArgs a, Range *out) {
+  const int64_t item = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> 6;
+  if (item >= int64_t(a.B) * a.tiles) return;
+  const int b = int(item / a.tiles), tile = int(item % a.tiles), lane = threadIdx.x & 63;
+  const int key = tile * kTile + lane;
+  const int n = place_of(a, b).n;
+  const int id = key < n ? a.documents[int64_t(b) * a.documents_stride + key] : -1;
+  int lo = id < 0 ? 0x7fffffff : id, hi = id < 0 ? -1 : id;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor(lo, o, 64));
+    hi = max(hi, __shfl_xor(hi, o, 64));
+  }
+  const bool full = __ballot(id < 0) == 0;
+  if (lane == 0) out[item] = Range{lo, hi, full, 0};
+}
+
+template <typename T> constexpr int pitch_pad() { return 16 / int(sizeof(T)); }
+
+// Rows [row0, row0 + 64) of a [rows][D] matrix into LDS, zero beyond its end and beyond D.
+template <typename T, int DP>
+__device__ __forceinline__ void load_tile(T *dst, const T *src, int64_t stride, int row0, int rows, int D, bool vec) {
+  constexpr int P = DP + pitch_pad<T>(), E = 16 / int(sizeof(T));
+  if (vec) {
+    typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+    for (int i = threadIdx.x; i < kTile * DP / E; i += 256) {
+      const int r = i / (DP / E), c = (i % (DP / E)) * E;
+      u32x4 v = {0, 0, 0, 0};
+      if (row0 + r < rows && c < D) v = *reinterpret_cast<const u32x4 *>(src + int64_t(row0 + r) * stride + c);
+      *reinterpret_cast<u32x4 *>(dst + r * P + c) = v;
+    }
+  } else {
+    for (int i = threadIdx.x; i < kTile * DP; i += 256) {
+      const int r = i / DP, c = i % DP;
+      dst[r * P + c] = row0 + r < rows && c < D ? src[int64_t(row0 + r) * stride + c] : T(0.f);
+    }
+  }
+}
+// The owned token's row as B fragments: d = 32 step + 8 grp + 0..7.
+template <typename T, int DP>
+__device__ __forceinline__ void load_own(typename Frag<T>::type (&f)[DP / 32], const T *row, int D, bool valid, int grp) {
+#pragma unroll
+  for (int st = 0; st < DP / 32; ++st) {
+    T t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = st * 32 + grp * 8 + e;
+      t[e] = valid && d < D ? row[d] : T(0.f);
+    }
+    __builtin_memcpy(&f[st], t, sizeof(t));
+  }
+}
+// Product of the tile's 64 rows with the owned columns: acc[kt][e] is row 16 kt + 4 grp + e.
+template <typename T, int DP>
+__device__ __forceinline__ void tile_product(const T *tile, const typename Frag<T>::type (&own)[DP / 32], f32x4 (&acc)[4]) {
+  constexpr int P = DP + pitch_pad<T>();
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) {
+    acc[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int st = 0; st < DP / 32; ++st) {
+      typename Frag<T>::type f;
+      __builtin_memcpy(&f, tile + (kt * 16 + col) * P + st * 32 + grp * 8, sizeof(f));
+      acc[kt] = mfma16(f, own[st], acc[kt]);
+    }
+  }
+}
+
+template <typename T> __device__ __forceinline__ bool finite(T x) { return fabsf(to_f32(x)) < INFINITY; }
+
+// acc[t] (rows 16 t + 4 grp + e of the result) += tile^T w, w the 64 rows' weights of this column.
+// strict: elements that are not finite count as 0 here and are then added where `seen` (bit 4 kt + e)
+// says so: an infinity as itself when `weights` says that w >= 0, else as NaN.
+template <typename T, int DP>
+__device__ __forceinline__ void add_transposed(const T *tile, const float (&w)[4][4], uint32_t seen, bool strict,
+                                               bool weights, f32x4 (&acc)[DP / 16]) {
+  constexpr int P = DP + pitch_pad<T>();
+  typedef typename Frag<T>::type F;
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    T wt[8], st[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      wt[e] = from_f32<T>(w[2 * c][e]);
+      wt[4 + e] = from_f32<T>(w[2 * c + 1][e]);
+      st[e] = T((seen >> (8 * c + e)) & 1 ? 1.f : 0.f);
+      st[4 + e] = T((seen >> (8 * c + 4 + e)) & 1 ? 1.f : 0.f);
+    }
+    F wf, sf;
+    __builtin_memcpy(&wf, wt, sizeof(wt));
+    __builtin_memcpy(&sf, st, sizeof(st));
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+      T at[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        at[e] = tile[(c * 32 + grp * 4 + e) * P + t * 16 + col];
+        at[4 + e] = tile[(c * 32 + 16 + grp * 4 + e) * P + t * 16 + col];
+      }
+      F af;
+      if (strict) {
+        T up[8], down[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool bad = !finite(at[e]);
+          const float x = to_f32(at[e]);
+          up[e] = T(bad && !(weights && x < 0.f) ? 1.f : 0.f);
+          down[e] = T(bad && !(weights && x > 0.f) ? 1.f : 0.f);
+          if (bad) at[e] = T(0.f);
+        }
+        F uf, df;
+        __builtin_memcpy(&uf, up, sizeof(up));
+        __builtin_memcpy(&df, down, sizeof(down));
+        const f32x4 ups = mfma16(uf, sf, f32x4{0.f, 0.f, 0.f, 0.f}), downs = mfma16(df, sf, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (ups[e] > 0.f) acc[t][e] += INFINITY;
+          if (downs[e] > 0.f) acc[t][e] -= INFINITY;
+        }
+      }
+      __builtin_memcpy(&af, at, sizeof(at));
+      acc[t] = mfma16(af, wf, acc[t]);
+    }
+  }
+}
+
+__device__ __forceinline__ float column_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float column_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+// Score of a pair in log 2 units, and d(score)/d(dot) up to `scale`.
+template <typename T> struct Scorer {
+  float scale, cap, inv_cap, slope;                    // slope in log 2 units
+  __device__ __forceinline__ Scorer(const SequenceArgs &a, int h)
+      : scale(a.scale), cap(a.cap), inv_cap(a.cap > 0.f ? 1.0f / a.cap : 0.f), slope(a.slopes ? a.slopes[h] * kLog2e : 0.f) {}
+  __device__ __forceinline__ float operator()(const SequenceArgs &a, float dot, int pos, int key, float &factor) const {
+    float x = dot * scale;
+    factor = 1.f;
+    if (a.cap > 0.f) {
+      const float t = bend<T>(x * inv_cap);
+      factor = 1.f - t * t;
+      x = cap * t;
+    }
+    x *= kLog2e;
+    if (a.slopes) x -= slope * fabsf(float(pos - key));
+    return x;
+  }
+};
+
+// Which of the 64 tiles from tile `first` on a workgroup with queries [i0, i1] needs (bit = tile), and which
+// of these it sees whole.
+struct Visit { uint64_t need, whole; };
+__device__ __forceinline__ Visit visit_keys(const SequenceArgs &a, const Place &p, int b, int first, int low, int high,
+                                            const Range &mine) {
+  const int tile = first + int(threadIdx.x & 63), k0 = tile * kTile;
+  bool need = tile < a.tiles && k0 < high, whole = need && k0 + kTile <= low;
+  if (a.documents && need) {
+    const Range r = static_cast<const Range *>(a.ranges)[int64_t(b) * a.tiles + tile];
+    need = overlap(r, mine);
+    whole = whole && same_document(r, mine);
+  }
+  return {__ballot(need), __ballot(need && whole)};
+}
+
+struct Owner { int block, h, b; };
+// Query blocks from the last to the first (a causal mask gives the last the most work), heads fastest.
+__device__ __forceinline__ Owner owner_of(int blocks, int heads, int item) {
+  const int h = item % heads, rest = item / heads;
+  return {blocks - 1 - rest % blocks, h, rest / blocks};
+}
+
+template <typename T, int DP> __global__ __launch_bounds__(256) void forward_kernel(SequenceArgs a, int blocks, bool vec) {
+  constexpr int P = DP + pitch_pad<T>();
+  __shared__ __attribute__((aligned(16))) T ks[kTile * P], vs[kTile * P];
+  __shared__ int ids[kTile];
+  const Owner own = owner_of(blocks, a.H, blockIdx.x);
+  const int b = own.b, h = own.h, hk = h / (a.H / a.Hk);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
+  const Place place = place_of(a, b);
+  const int i0 = own.block * kTile, i1 = min(i0 + kTile, a.Nq) - 1, i = i0 + wave * 16 + col;
+  const bool valid = i < a.Nq;
+  const Row row = row_of(a, place, b, i);
+  const T *kp = static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[1];
+  const T *vp = static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[1];
+  typename Frag<T>::type qf[DP / 32];
+  load_own<T, DP>(qf, static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1] + i * a.qs[2], a.D, valid, grp);
+  const int low = limit_of(a, place, i0), high = limit_of(a, place, i1);
+  const Range mine = a.documents ? query_range(a, place, b, i0, i1) : Range{};
+  const Scorer<T> score(a, h);
+
+  f32x4 o[DP / 16];
+  float m, l;
+  for (int strict = 0; strict < 2; ++strict) {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int first = 0; first * kTile < high; first += 64) {
+      Visit visit = visit_keys(a, place, b, first, low, high, mine);
+      while (visit.need) {
+        const int bit = __builtin_ctzll(visit.need), k0 = (first + bit) * kTile;
+        const bool whole = (visit.whole >> bit) & 1;
+        visit.need &= visit.need - 1;
+        __syncthreads();
+        load_tile<T, DP>(ks, kp, a.ks[2], k0, place.n, a.D, vec);
+        load_tile<T, DP>(vs, vp, a.vs[2], k0, place.n, a.Dv, vec);
+        if (a.documents && tid < kTile) ids[tid] = k0 + tid < place.n ? a.documents[int64_t(b) * a.documents_stride + k0 + tid] : -1;
+        __syncthreads();
+        f32x4 s[4];
+        tile_product<T, DP>(ks, qf, s);
+        float w[4][4];
+        uint32_t seen = 0;
+        float top = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = kt * 16 + grp * 4 + e, key = k0 + r;
+            const bool see = whole || (key < row.limit && (!a.documents || ids[r] == row.document));
+            float factor;
+            const float x = score(a, s[kt][e], row.pos, key, factor);
+            w[kt][e] = x;
+            if (see) {
+              seen |= 1u << (4 * kt + e);
+              top = fmaxf(top, x);
+            }
+          }
+        const float m_new = fmaxf(m, column_max(top)), base = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = exp2_of<T>(m - base);
+        m = m_new;
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) o[t] *= alpha;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            w[kt][e] = (seen >> (4 * kt + e)) & 1 ? exp2_of<T>(w[kt][e] - base) : 0.f;
+            l += w[kt][e];
+          }
+        add_transposed<T, DP>(vs, w, seen, strict != 0, true, o);
+      }
+    }
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad |= !(fabsf(o[t][e]) < INFINITY);
+    if (!__syncthreads_or(valid && bad)) break;
+  }
+  l = column_sum(l);
+  if (!valid) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  T *op = static_cast<T *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2];
+#pragma unroll
+  for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = t * 16 + grp * 4 + e;
+      if (d < a.Dv) op[d] = from_f32<T>(o[t][e] * inv);
+    }
+  if (a.lse && grp == 0) a.lse[(int64_t(b) * a.H + h) * a.Nq + i] = l == 0.f ? INFINITY : m + log2f(l);
+}
+
+// dq of 64 queries, their delta = dout . out (for dk and dv), and the slopes' part:
+//   d slope = - sum_j dS_ij |p_i - j| = - (sum_j P dP |.| - (sum_j P dP) (sum_j P |.|)) for each query,
+// its three sums in fp32 and from unrounded values (delta, which has the rounded output in it, is kept out).
+template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(SequenceArgs a, int blocks, bool vec) {
+  constexpr int P = DP + pitch_pad<T>();
+  __shared__ __attribute__((aligned(16))) T ks[kTile * P], vs[kTile * P];
+  __shared__ int ids[kTile];
+  __shared__ float part[kTile];
+  const Owner own = owner_of(blocks, a.H, blockIdx.x);
+  const int b = own.b, h = own.h, hk = h / (a.H / a.Hk);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
+  const Place place = place_of(a, b);
+  const int i0 = own.block * kTile, i1 = min(i0 + kTile, a.Nq) - 1, i = i0 + wave * 16 + col;
+  const bool valid = i < a.Nq;
+  const Row row = row_of(a, place, b, i);
+  const T *kp = static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[1];
+  const T *vp = static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[1];
+  typename Frag<T>::type qf[DP / 32], gf[DP / 32];
+  load_own<T, DP>(qf, static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1] + i * a.qs[2], a.D, valid, grp);
+  const T *gp = static_cast<const T *>(a.dout) + b * a.gs[0] + h * a.gs[1] + i * a.gs[2];
+  const T *op = static_cast<const T *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2];
+  load_own<T, DP>(gf, gp, a.Dv, valid, grp);
+  float delta = 0.f;
+  if (valid)
+    for (int d0 = grp * 8; d0 < a.Dv; d0 += 32)
+      for (int d = d0; d < min(d0 + 8, a.Dv); ++d) delta += to_f32(gp[d]) * to_f32(op[d]);
+  delta = column_sum(delta);
+  const int64_t at = (int64_t(b) * a.H + h) * a.Nq + i;
+  const float lse = valid ? a.lse[at] : INFINITY;
+  if (valid && grp == 0) a.delta[at] = delta;
+  const int low = limit_of(a, place, i0), high = limit_of(a, place, i1);
+  const Range mine = a.documents ? query_range(a, place, b, i0, i1) : Range{};
+  const Scorer<T> score(a, h);
+
+  f32x4 dq[DP / 16];
+  float far_dp, far, pdp;
+  for (int strict = 0; strict < 2; ++strict) {
+    far_dp = far = pdp = 0.f;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) dq[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int first = 0; first * kTile < high; first += 64) {
+      Visit visit = visit_keys(a, place, b, first, low, high, mine);
+      while (visit.need) {
+        const int bit = __builtin_ctzll(visit.need), k0 = (first + bit) * kTile;
+        const bool whole = (visit.whole >> bit) & 1;
+        visit.need &= visit.need - 1;
+        __syncthreads();
+        load_tile<T, DP>(ks, kp, a.ks[2], k0, place.n, a.D, vec);
+        load_tile<T, DP>(vs, vp, a.vs[2], k0, place.n, a.Dv, vec);
+        if (a.documents && tid < kTile) ids[tid] = k0 + tid < place.n ? a.documents[int64_t(b) * a.documents_stride + k0 + tid] : -1;
+        __syncthreads();
+        f32x4 s[4], dp[4];
+        tile_product<T, DP>(ks, qf, s);
+        tile_product<T, DP>(vs, gf, dp);
+        float w[4][4];
+        uint32_t seen = 0;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = kt * 16 + grp * 4 + e, key = k0 + r;
+            const bool see = valid && (whole || (key < row.limit && (!a.documents || ids[r] == row.document)));
+            float factor;
+            const float x = score(a, s[kt][e], row.pos, key, factor);
+            const float p = see ? exp2_of<T>(x - lse) : 0.f;
+            w[kt][e] = see ? p * (dp[kt][e] - delta) * factor : 0.f;
+            seen |= see ? 1u << (4 * kt + e) : 0u;
+            if (a.slope_part && see) {
+              const float gap = fabsf(float(row.pos - key));
+              pdp += p * dp[kt][e];
+              far += p * gap;
+              far_dp += p * dp[kt][e] * gap;
+            }
+          }
+        add_transposed<T, DP>(ks, w, seen, strict != 0, false, dq);
+      }
+    }
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad |= !(fabsf(dq[t][e]) < INFINITY);
+    if (!__syncthreads_or(valid && bad)) break;
+  }
+  if (valid) {
+    T *out = static_cast<T *>(a.dq) + b * a.dqs[0] + h * a.dqs[1] + i * a.dqs[2];
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = t * 16 + grp * 4 + e;
+        if (d < a.D) out[d] = from_f32<T>(dq[t][e] * a.scale);
+      }
+  }
+  if (a.slope_part) {
+    far_dp = column_sum(far_dp);
+    far = column_sum(far);
+    pdp = column_sum(pdp);
+    if (grp == 0) part[wave * 16 + col] = valid ? -(far_dp - pdp * far) : 0.f;
+    __syncthreads();
+    if (tid < kTile) {
+      const float t = wave_sum(part[tid]);
+      if (tid == 0) a.slope_part[(int64_t(h) * a.B + b) * blocks + own.block] = t;
+    }
+  }
+}
+
+// dk and dv of 64 keys: over the heads that share them and the queries that see them.
+template <typename T, int DP> __global__ __launch_bounds__(256) void dkv_kernel(SequenceArgs a, int blocks, bool vec) {
+  constexpr int P = DP + pitch_pad<T>();
+  __shared__ __attribute__((aligned(16))) T qs[kTile * P], gs[kTile * P];
+  __shared__ Row rows[kTile];
+  __shared__ float lses[kTile], deltas[kTile];
+  const int hk = blockIdx.x % a.Hk, rest = blockIdx.x / a.Hk, group = a.H / a.Hk;
+  const int block = rest % blocks, b = rest / blocks;      // the first keys, which causal queries see most, first
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
+  const Place place = place_of(a, b);
+  const int k0 = block * kTile, key = k0 + wave * 16 + col;
+  const bool valid = key < place.n;
+  typename Frag<T>::type kf[DP / 32], vf[DP / 32];
+  load_own<T, DP>(kf, static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[1] + key * a.ks[2], a.D, valid, grp);
+  load_own<T, DP>(vf, static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[1] + key * a.vs[2], a.Dv, valid, grp);
+  int id = 0;
+  Range mine{};
+  if (a.documents) {
+    id = valid ? a.documents[int64_t(b) * a.documents_stride + key] : -1;
+    mine = static_cast<const Range *>(a.ranges)[int64_t(b) * a.tiles + block];
+  }
+  const int qtiles = (a.Nq + kTile - 1) / kTile;
+
+  f32x4 dk[DP / 16], dv[DP / 16];
+  for (int strict = 0; strict < 2; ++strict) {
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) dk[t] = dv[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < group; ++g) {
+      const int h = hk * group + g;
+      const T *qp = static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1];
+      const T *gp = static_cast<const T *>(a.dout) + b * a.gs[0] + h * a.gs[1];
+      const Scorer<T> score(a, h);
+      const int64_t at = (int64_t(b) * a.H + h) * a.Nq;
+      for (int first = 0; first < qtiles; first += 64) {
+        const int tile = first + lane, r0 = tile * kTile, r1 = min(r0 + kTile, a.Nq) - 1;
+        bool need = tile < qtiles && limit_of(a, place, r1) > k0, whole = need && limit_of(a, place, r0) >= k0 + kTile;
+        if (a.documents && need) {
+          const Range r = query_range(a, place, b, r0, r1);
+          need = overlap(r, mine);
+          whole = whole && same_document(r, mine);
+        }
+        uint64_t todo = __ballot(need);
+        const uint64_t wholes = __ballot(need && whole && r0 + kTile <= a.Nq);
+        while (todo) {
+          const int bit = __builtin_ctzll(todo), i0 = (first + bit) * kTile;
+          const bool all = (wholes >> bit) & 1;
+          todo &= todo - 1;
+          __syncthreads();
+          load_tile<T, DP>(qs, qp, a.qs[2], i0, a.Nq, a.D, vec);
+          load_tile<T, DP>(gs, gp, a.gs[2], i0, a.Nq, a.Dv, vec);
+          if (tid < kTile) {
+            const int i = i0 + tid;
+            rows[tid] = row_of(a, place, b, i);
+            lses[tid] = i < a.Nq ? a.lse[at + i] : INFINITY;
+            deltas[tid] = i < a.Nq ? a.delta[at + i] : 0.f;
+          }
+          __syncthreads();
+          f32x4 s[4], dp[4];
+          tile_product<T, DP>(qs, kf, s);
+          tile_product<T, DP>(gs, vf, dp);
+          float pw[4][4], w[4][4];
+          uint32_t seen = 0;
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = kt * 16 + grp * 4 + e;
+              const Row row = rows[r];
+              const bool see = valid && (all || (key < row.limit && (!a.documents || id == row.document)));
+              float factor;
+              const float x = score(a, s[kt][e], row.pos, key, factor);
+              pw[kt][e] = see ? exp2_of<T>(x - lses[r]) : 0.f;
+              w[kt][e] = see ? pw[kt][e] * (dp[kt][e] - deltas[r]) * factor : 0.f;
+              seen |= see ? 1u << (4 * kt + e) : 0u;
+            }
+          add_transposed<T, DP>(gs, pw, seen, strict != 0, false, dv);
+          add_transposed<T, DP>(qs, w, seen, strict != 0, false, dk);
+        }
+      }
+    }
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad |= !(fabsf(dk[t][e]) < INFINITY) || !(fabsf(dv[t][e]) < INFINITY);
+    if (!__syncthreads_or(valid && bad)) break;
+  }
+  if (key >= a.Nk) return;                                 // (keys beyond a length: zeros)
+  T *kout = static_cast<T *>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2];
+  T *vout = static_cast<T *>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2];
+#pragma unroll
+  for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = t * 16 + grp * 4 + e;
+      if (d < a.D) kout[d] = from_f32<T>(valid ? dk[t][e] * a.scale : 0.f);
+      if (d < a.Dv) vout[d] = from_f32<T>(valid ? dv[t][e] : 0.f);
+    }
+}
+
+// dslopes[h]: the sum of its parts, in their order.
+__global__ __launch_bounds__(256) void dslopes_kernel(const float *part, int64_t count, float *out) {
+  __shared__ double sums[256];
+  double t = 0.0;
+  for (int64_t i = threadIdx.x; i < count; i += 256) t += double(part[blockIdx.x * count + i]);
+  sums[threadIdx.x] = t;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (int(threadIdx.x) < o) sums[threadIdx.x] += sums[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) out[blockIdx.x] = float(sums[0]);
+}
+
+// Rows that can be read 16 bytes at a time.
+template <typename T> bool vector_rows(std::initializer_list<std::pair<const void *, const int64_t *>> tensors, int64_t D) {
+  constexpr int64_t E = 16 / sizeof(T);
+  if (D % E) return false;
+  for (const auto &t : tensors)
+    if (reinterpret_cast<uintptr_t>(t.first) % 16 || t.second[0] % E || t.second[1] % E || t.second[2] % E) return false;
+  return true;
+}
+
+template <typename T, int DP> int launch_forward(const SequenceArgs &a, hipStream_t s) {
+  const int64_t blocks = ceil_div(a.Nq, int64_t(kTile));
+  const bool vec = vector_rows<T>({{a.k, a.ks}}, a.D) && vector_rows<T>({{a.v, a.vs}}, a.Dv);
+  forward_kernel<T, DP><<<dim3(unsigned(blocks * a.H * a.B)), 256, 0, s>>>(a, int(blocks), vec);
+  return check_launch("sequence_attention");
+}
+
+template <typename T, int DP> int launch_backward(const SequenceArgs &a, hipStream_t s) {
+  const int64_t qblocks = ceil_div(a.Nq, int64_t(kTile)), kblocks = ceil_div(a.Nk, int64_t(kTile));
+  const bool vec = vector_rows<T>({{a.k, a.ks}, {a.q, a.qs}}, a.D) && vector_rows<T>({{a.v, a.vs}, {a.dout, a.gs}}, a.Dv);
+  if (qblocks > 0 && a.H > 0) dq_kernel<T, DP><<<dim3(unsigned(qblocks * a.H * a.B)), 256, 0, s>>>(a, int(qblocks), vec);
+  XFH_TRY(check_launch("sequence_attention_backward"));
+  if (kblocks > 0) dkv_kernel<T, DP><<<dim3(unsigned(kblocks * a.Hk * a.B)), 256, 0, s>>>(a, int(kblocks), vec);
+  return check_launch("sequence_attention_backward");
+}
+
+int check_grid(const SequenceArgs &a) {
+  const int64_t most = std::max(ceil_div(int64_t(a.Nq), int64_t(kTile)) * a.H, ceil_div(int64_t(a.Nk), int64_t(kTile)) * a.Hk) * a.B;
+  if (most > (int64_t(1) << 31) - 1) return fail(XFH_EUNSUPPORTED, "sequence_attention: problem too large");
+  return XFH_OK;
+}
+
+}  // namespace
+
+int64_t sequence_ranges_bytes(int64_t B, int64_t Nk) { return B * ceil_div(Nk, int64_t(kTile)) * int64_t(sizeof(Range)); }
+
+int sequence_ranges(const SequenceArgs &a, hipStream_t s) {
+  const int64_t items = int64_t(a.B) * a.tiles;
+  if (!a.documents || items == 0) return XFH_OK;
+  if (ceil_div(items, int64_t(4)) > (int64_t(1) << 31) - 1) return fail(XFH_EUNSUPPORTED, "sequence_attention: problem too large");
+  ranges_kernel<<<dim3(unsigned(ceil_div(items, int64_t(4)))), 256, 0, s>>>(a, static_cast<Range *>(const_cast<void *>(a.ranges)));
+  return check_launch("sequence_attention");
+}
+
+int sequence_forward(const SequenceArgs &a, int dtype, hipStream_t s) {
+  if (a.B == 0 || a.H == 0 || a.Nq == 0) return XFH_OK;
+  XFH_TRY(check_grid(a));
+  XFH_TRY(sequence_ranges(a, s));
+  const int d = std::max(a.D, a.Dv);
+#define XFH_SEQ_FORWARD(DP) return dtype == XFH_BF16 ? launch_forward<bf16, DP>(a, s) : launch_forward<float, DP>(a, s)
+  if (d <= 32) XFH_SEQ_FORWARD(32);
+  if (d <= 64) XFH_SEQ_FORWARD(64);
+  if (d <= 96) XFH_SEQ_FORWARD(96);
+  XFH_SEQ_FORWARD(128);
+#undef XFH_SEQ_FORWARD
+}
+
+int64_t sequence_slope_part(int64_t B, int64_t H, int64_t Nq) { return H * B * ceil_div(Nq, int64_t(kTile)); }
+
+int sequence_backward(const SequenceArgs &a, int dtype, float *dslopes, hipStream_t s) {
+  if (a.B > 0 && a.Hk > 0) {
+    XFH_TRY(check_grid(a));
+    XFH_TRY(sequence_ranges(a, s));
+    const int d = std::max(a.D, a.Dv);
+    int status = XFH_OK;
+#define XFH_SEQ_BACKWARD(DP) status = dtype == XFH_BF16 ? launch_backward<bf16, DP>(a, s) : launch_backward<float, DP>(a, s)
+    if (d <= 32) XFH_SEQ_BACKWARD(32);
+    else if (d <= 64) XFH_SEQ_BACKWARD(64);
+    else if (d <= 96) XFH_SEQ_BACKWARD(96);
+    else XFH_SEQ_BACKWARD(128);
+#undef XFH_SEQ_BACKWARD
+    if (status != XFH_OK) return status;
+  }
+  if (!dslopes || a.H == 0) return XFH_OK;
+  dslopes_kernel<<<dim3(unsigned(a.H)), 256, 0, s>>>(a.slope_part, int64_t(a.B) * ceil_div(int64_t(a.Nq), int64_t(kTile)), dslopes);
+  return check_launch("sequence_attention_backward");
+}
+
+}  // namespace xfh

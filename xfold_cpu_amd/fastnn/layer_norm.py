@@ -1,16 +1,109 @@
 """LayerNorm module with the reference's constructor and parameters
 (``xfold/fastnn/layer_norm.py:14-53``), dispatching on ``config.layer_norm_implementation``
-(``layer_norm.py:55-81``); this package implements the ``"hip"`` value."""
+(``layer_norm.py:55-81``); this package implements the ``"hip"`` value. In training mode the module
+is :func:`trainable_layer_norm`, which has a backward pass."""
 
 from __future__ import annotations
 
 import numbers
+from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import config as fastnn_config
+from . import native_hip as nh
 from . import ops
+
+
+def _rows(t: torch.Tensor, cols: int):
+    """(``t``, or a contiguous copy of it, and its stride between rows of ``cols`` elements)."""
+    if not t.is_contiguous():
+        if t.dim() == 2 and t.shape[1] == cols and t.stride(1) == 1 and t.stride(0) >= cols:
+            return t, t.stride(0)
+        t = t.contiguous()
+    return t, cols
+
+
+def _forward(x, cols, weight, bias, eps, out_dtype, keep):
+    x, stride = _rows(x, cols)
+    rows = x.numel() // cols if cols else 0
+    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if keep else None
+    with nh.on_device(x.device):
+        nh.call("xfh_layer_norm_train", nh.ptr(x), nh.dtype_code(x.dtype), stride, rows, cols, nh.ptr(weight),
+                nh.F32 if weight is None else nh.dtype_code(weight.dtype), nh.ptr(bias),
+                nh.F32 if bias is None else nh.dtype_code(bias.dtype), eps, nh.ptr(y), nh.dtype_code(out_dtype),
+                nh.ptr(stats), nh.stream_of(x.device))
+    return x, y, stats
+
+
+class _TrainableLayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, cols, eps, out_dtype):
+        w = None if weight is None else weight.contiguous()
+        x, y, stats = _forward(x, cols, w, None if bias is None else bias.contiguous(), eps, out_dtype, True)
+        ctx.save_for_backward(x, w, stats)
+        ctx.cols, ctx.out_dtype = cols, out_dtype
+        ctx.bias_of = None if bias is None else (bias.shape, bias.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        cols, device = ctx.cols, x.device
+        if dy.dtype != ctx.out_dtype:
+            dy = dy.to(ctx.out_dtype)
+        dy, dy_stride = _rows(dy, cols)
+        x, x_stride = _rows(x, cols)
+        rows = x.numel() // cols if cols else 0
+        dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty(ctx.bias_of[0], dtype=ctx.bias_of[1], device=device) if need_b else None
+        with nh.on_device(device):
+            ws = None
+            if need_w or need_b:
+                ws = nh.workspace(nh.load_library().xfh_layer_norm_backward_workspace_size(rows, cols), device)
+            nh.call("xfh_layer_norm_backward", nh.ptr(dy), nh.dtype_code(dy.dtype), dy_stride, nh.ptr(x),
+                    nh.dtype_code(x.dtype), x_stride, rows, cols, nh.ptr(weight),
+                    nh.F32 if weight is None else nh.dtype_code(weight.dtype), nh.ptr(stats), nh.ptr(dx), nh.ptr(dw),
+                    nh.F32 if dw is None else nh.dtype_code(dw.dtype), nh.ptr(db),
+                    nh.F32 if db is None else nh.dtype_code(db.dtype), nh.ptr(ws), 0 if ws is None else ws.numel(),
+                    nh.stream_of(device))
+        return dx, dw, db, None, None, None
+
+
+def trainable_layer_norm(x: torch.Tensor, normalized_shape, weight: Optional[torch.Tensor] = None,
+                         bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """F.layer_norm over the trailing ``normalized_shape``, with gradients of ``x``, ``weight`` and
+    ``bias`` (once; the backward pass itself is not differentiable). FP32/BF16 input, weight and bias,
+    each in a type of its own; statistics and sums in FP32. As with :class:`LayerNorm` in eval mode the
+    output is in the input's type, under autocast in FP32 (``xfold/fastnn/layer_norm.py:56-59``)."""
+    if fastnn_config.layer_norm_implementation != fastnn_config.HIP:
+        raise ValueError("xfold_cpu_amd implements layer_norm_implementation='hip' only, "
+                         f"got {fastnn_config.layer_norm_implementation!r}")
+    nh.check_gpu(x, weight, bias)
+    if any(t is not None and t.dtype not in (torch.float32, torch.bfloat16) for t in (x, weight, bias)):
+        raise ValueError("The 'hip' LayerNorm supports FP32/BF16 tensors.")
+    shape = (normalized_shape,) if isinstance(normalized_shape, numbers.Integral) else tuple(normalized_shape)
+    if not shape or tuple(x.shape[x.dim() - len(shape):]) != shape:
+        raise ValueError(f"LayerNorm: input shape {tuple(x.shape)} does not end with {shape}.")
+    if any(t is not None and tuple(t.shape) != shape for t in (weight, bias)):
+        raise ValueError(f"LayerNorm: weight and bias must have the shape {shape}.")
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError("LayerNorm: eps must be nonnegative.")
+    cols = 1
+    for s in shape:
+        cols *= s
+    out_dtype = torch.float32 if torch.is_autocast_enabled("cuda") else x.dtype
+    if nh.needs_gradient(x, weight, bias):
+        return _TrainableLayerNorm.apply(x, weight, bias, cols, eps, out_dtype)
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    return _forward(x, cols, weight, bias, eps, out_dtype, False)[1]
 
 
 class LayerNorm(nn.Module):
@@ -38,7 +131,7 @@ class LayerNorm(nn.Module):
             raise ValueError("xfold_cpu_amd implements layer_norm_implementation='hip' only, "
                              f"got {fastnn_config.layer_norm_implementation!r}")
         if self.training:
-            raise RuntimeError("The 'hip' LayerNorm supports eval inference only.")
+            return trainable_layer_norm(input, self.normalized_shape, self.weight, self.bias, self.eps)
         return ops.layer_norm(input, self.normalized_shape, self.weight, self.bias, self.eps, owner=self)
 
     def extra_repr(self) -> str:

@@ -19,6 +19,7 @@ runs in the library's HIP kernels.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -28,7 +29,7 @@ from typing import Optional
 import torch
 
 LIBRARY_PATH = Path(__file__).resolve().parent.parent / "lib" / "libxfold_hip.so"
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 F32, BF16, BOOL = 0, 1, 2
 BIAS_PACKED = 3                 # bias 'dtype' of a packed fp32 block (times log2(e))
@@ -48,6 +49,14 @@ SIGNATURES = {
     "xfh_kernel_timing_read_work": (_i, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double), _pi64,
                                          ctypes.POINTER(ctypes.c_double)]),
     "xfh_layer_norm": (_i, [_p, _i, _i64, _i64, _p, _p, _f, _p, _i, _p]),
+    "xfh_layer_norm_train": (_i, [_p, _i, _i64, _i64, _i64, _p, _i, _p, _i, _f, _p, _i, _p, _p]),
+    "xfh_layer_norm_backward_workspace_size": (_i64, [_i64, _i64]),
+    "xfh_layer_norm_backward": (_i, [_p, _i, _i64, _p, _i, _i64, _i64, _i64, _p, _i, _p, _p, _p, _i, _p, _i, _p, _i64,
+                                     _p]),
+    "xfh_sequence_attention_workspace_size": (_i64, [_p]),
+    "xfh_sequence_attention": (_i, [_p, _p, _i64, _p]),
+    "xfh_sequence_attention_backward_workspace_size": (_i64, [_p]),
+    "xfh_sequence_attention_backward": (_i, [_p, _p, _i64, _p]),
     "xfh_adaptive_layer_norm": (_i, [_p, _i, _i64, _i64, _p, _p, _i, _i64, _f, _p, _i, _p]),
     "xfh_linear": (_i, [_p, _i64, _p, _p, _i64, _i64, _i64, _i, _p, _i64, _i, _i, _p, _i64, _i64, _p]),
     "xfh_linear_batched": (_i, [_p, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i, _p, _i64, _i64, _i, _p]),
@@ -131,6 +140,18 @@ class DiffusionBlock(ctypes.Structure):
                ("attention_eps", ctypes.c_float), ("transition_eps", ctypes.c_float)]
 
 
+class SequenceAttention(ctypes.Structure):
+    """``XfhSequenceAttention`` of include/xfold_hip.h, its strides one by one."""
+    _fields_ = [(name, ctypes.c_void_p) for name in
+                ("q", "k", "v", "out", "lse", "slopes", "prefix", "documents", "lengths", "dout", "dq", "dk", "dv",
+                 "dslopes")] + [
+               (name, ctypes.c_int64) for name in
+               ("batch", "heads", "kv_heads", "queries", "keys", "dim", "value_dim",
+                *(f"{t}_{s}" for t in ("q", "k", "v", "out", "dout", "dq", "dk", "dv") for s in ("batch", "head", "token")),
+                "documents_stride", "prefix_all")] + [
+               ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("causal", ctypes.c_int), ("dtype", ctypes.c_int)]
+
+
 def call(name: str, *args) -> None:
     lib = load_library()
     status = getattr(lib, name)(*args)
@@ -194,6 +215,30 @@ def check_gpu_inference(*tensors) -> None:
             raise RuntimeError("The 'hip' backend supports inference only; disable gradients.")
         if tensor.device.type != "cuda" or tensor.layout != torch.strided:
             raise ValueError("The 'hip' backend requires strided ROCm (cuda) tensors.")
+
+
+def check_gpu(*tensors) -> torch.device:
+    """Device and layout guards of the operators that have a backward pass: strided ROCm tensors, all
+    on one device, which is returned."""
+    device = None
+    for tensor in tensors:
+        if tensor is None:
+            continue
+        if tensor.device.type != "cuda" or tensor.layout != torch.strided:
+            raise ValueError("The 'hip' backend requires strided ROCm (cuda) tensors.")
+        if device is not None and tensor.device != device:
+            raise ValueError(f"The 'hip' backend requires tensors on one device, got {device} and {tensor.device}.")
+        device = tensor.device
+    return device
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` the current one while a call is launched (nothing where it is already)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def needs_gradient(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def compute_dtype(x: torch.Tensor, *weights: torch.Tensor) -> torch.dtype:
