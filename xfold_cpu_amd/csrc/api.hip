@@ -973,9 +973,11 @@ static int sequence_args(const XfhSequenceAttention *p, SequenceArgs &a) {
   return XFH_OK;
 }
 
-struct SequencePlan { void *ranges; float *delta, *slope_part; };
-static int64_t sequence_carve(Carver &cv, SequencePlan &p, const SequenceArgs &a, bool backward, bool slopes) {
+struct SequencePlan { void *ranges, *parts; int splits; float *delta, *slope_part; };
+static int64_t sequence_carve(Carver &cv, SequencePlan &p, const SequenceArgs &a, int dtype, bool backward, bool slopes) {
   std::memset(&p, 0, sizeof(p));
+  p.splits = !backward && dtype == XFH_BF16 ? sequence_splits(a.B, a.H, a.Hk, a.Nq, a.Nk) : 1;
+  if (p.splits > 1) p.parts = cv.take(sequence_parts_bytes(a.B, a.H, a.Nq, a.Dv, p.splits));
   if (a.documents) p.ranges = cv.take(sequence_ranges_bytes(a.B, a.Nk));
   if (backward) {
     p.delta = static_cast<float *>(cv.take(int64_t(a.B) * a.H * a.Nq * 4));
@@ -992,7 +994,7 @@ int64_t xfh_sequence_attention_workspace_size(const XfhSequenceAttention *args) 
   SequenceArgs a;
   SequencePlan p;
   Carver cv(nullptr, 0);
-  return sequence_args(args, a) == XFH_OK ? sequence_carve(cv, p, a, false, false) : -1;
+  return sequence_args(args, a) == XFH_OK ? sequence_carve(cv, p, a, args->dtype, false, false) : -1;
 }
 
 int xfh_sequence_attention(const XfhSequenceAttention *args, void *workspace, int64_t workspace_bytes, void *stream) {
@@ -1002,17 +1004,17 @@ int xfh_sequence_attention(const XfhSequenceAttention *args, void *workspace, in
   if (a.B == 0 || a.H == 0 || a.Nq == 0) return XFH_OK;
   XFH_REQUIRE(a.q && a.out && (a.Nk == 0 || (a.k && a.v)), "sequence_attention: null tensor");
   Carver cv(workspace, workspace_bytes);
-  if (sequence_carve(cv, p, a, false, false) > (workspace ? workspace_bytes : 0))
+  if (sequence_carve(cv, p, a, args->dtype, false, false) > (workspace ? workspace_bytes : 0))
     return fail(XFH_EWORKSPACE, "sequence_attention: workspace too small (need " + std::to_string(cv.used) + " bytes)");
   a.ranges = p.ranges;
-  return sequence_forward(a, args->dtype, as_stream(stream));
+  return sequence_forward(a, args->dtype, p.parts, p.splits, as_stream(stream));
 }
 
 int64_t xfh_sequence_attention_backward_workspace_size(const XfhSequenceAttention *args) {
   SequenceArgs a;
   SequencePlan p;
   Carver cv(nullptr, 0);
-  return sequence_args(args, a) == XFH_OK ? sequence_carve(cv, p, a, true, args->dslopes != nullptr) : -1;
+  return sequence_args(args, a) == XFH_OK ? sequence_carve(cv, p, a, args->dtype, true, args->dslopes != nullptr) : -1;
 }
 
 int xfh_sequence_attention_backward(const XfhSequenceAttention *args, void *workspace, int64_t workspace_bytes, void *stream) {
@@ -1024,7 +1026,7 @@ int xfh_sequence_attention_backward(const XfhSequenceAttention *args, void *work
   XFH_REQUIRE(!queries || (a.q && a.out && a.lse && a.dout && a.dq), "sequence_attention_backward: null tensor");
   XFH_REQUIRE(!keys || (a.k && a.v && a.dk && a.dv), "sequence_attention_backward: null tensor");
   Carver cv(workspace, workspace_bytes);
-  if (sequence_carve(cv, p, a, true, args->dslopes != nullptr) > (workspace ? workspace_bytes : 0))
+  if (sequence_carve(cv, p, a, args->dtype, true, args->dslopes != nullptr) > (workspace ? workspace_bytes : 0))
     return fail(XFH_EWORKSPACE, "sequence_attention_backward: workspace too small (need " + std::to_string(cv.used) + " bytes)");
   a.ranges = p.ranges;
   a.delta = p.delta;

@@ -305,7 +305,7 @@ struct SequenceArgs {
   void *out, *dq, *dk, *dv;
   float *lse;                // [B][H][Nq], log2 of the sum of exp2 of the scores; +inf: no visible key
   float *delta;              // [B][H][Nq], dout . out
-  float *slope_part;         // [H][B][query tiles], or null
+  float *slope_part;         // [H][B][Nq], or null
   const float *slopes;       // [H], or null
   const int32_t *prefix, *documents, *lengths;
   const void *ranges;        // [B][tiles] seq::Range, with documents
@@ -317,7 +317,14 @@ struct SequenceArgs {
 };
 int64_t sequence_ranges_bytes(int64_t B, int64_t Nk);
 int sequence_ranges(const SequenceArgs &a, hipStream_t s);
-int sequence_forward(const SequenceArgs &a, int dtype, hipStream_t s);
+// bf16 (sequence_bf16.hip): the keys of a forward pass with few workgroups are split, their parts joined.
+int sequence_splits(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk);
+int64_t sequence_parts_bytes(int64_t B, int64_t H, int64_t Nq, int64_t Dv, int splits);
+bool sequence_bf16_forward_fits(const SequenceArgs &a);
+bool sequence_bf16_backward_fits(const SequenceArgs &a);
+int sequence_bf16_forward(const SequenceArgs &a, void *parts, int splits, hipStream_t s);
+int sequence_bf16_backward(const SequenceArgs &a, hipStream_t s);
+int sequence_forward(const SequenceArgs &a, int dtype, void *parts, int splits, hipStream_t s);
 int64_t sequence_slope_part(int64_t B, int64_t H, int64_t Nq);   // floats
 int sequence_backward(const SequenceArgs &a, int dtype, float *dslopes, hipStream_t s);
 

@@ -47,16 +47,17 @@ __device__ __forceinline__ Row row_of(const SequenceArgs &a, const Place &p, int
   return r;
 }
 
-// Range of the documents of queries [i0, i1] (at most 64 of them: they lie in two tiles).
+// Range of the documents of queries [i0, i1].
 __device__ __forceinline__ Range query_range(const SequenceArgs &a, const Place &p, int b, int i0, int i1) {
   const int p0 = max(i0 + p.shift, 0), p1 = i1 + p.shift;
   if (p1 < 0) return Range{0x7fffffff, -1, 0, 0};
   const Range *r = static_cast<const Range *>(a.ranges) + int64_t(b) * a.tiles;
   Range u = r[p0 / kTile];
-  const Range w = r[p1 / kTile];
-  u.x = min(u.x, w.x);
-  u.y = max(u.y, w.y);
-  u.z = u.z & w.z;
+  for (int t = p0 / kTile + 1; t <= p1 / kTile; ++t) {
+    u.x = min(u.x, r[t].x);
+    u.y = max(u.y, r[t].y);
+    u.z &= r[t].z;
+  }
   return u;
 }
 __device__ __forceinline__ bool overlap(const Range &u, const Range &w) { return u.x <= w.y && w.x <= u.y; }

@@ -1,4 +1,5 @@
-// Sequence attention for any head dim up to 128 in bf16 and fp32: forward, dq, dk and dv.
+// Sequence attention for any head dim up to 128, in fp32 and for the bf16 layouts that sequence_bf16.hip does
+// not take (rows that are not whole 16-byte pieces): forward, dq, dk and dv.
 //
 // A workgroup owns 64 tokens (16 per wavefront, one per lane column): queries in the forward pass and
 // for dq, keys for dk and dv. It walks the other side in tiles of 64, held row-major in LDS. With the
@@ -299,14 +300,13 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void forward_ker
   if (a.lse && grp == 0) a.lse[(int64_t(b) * a.H + h) * a.Nq + i] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
-// dq of 64 queries, their delta = dout . out (for dk and dv), and the slopes' part:
-//   d slope = - sum_j dS_ij |p_i - j| = - (sum_j P dP |.| - (sum_j P dP) (sum_j P |.|)) for each query,
-// its three sums in fp32 and from unrounded values (delta, which has the rounded output in it, is kept out).
+// dq of 64 queries, their delta = dout . out (for dk and dv), and the slopes' part of each query,
+//   - sum_j P (dP - sum P dP) |gap| = - (sum_j P (dP - delta) |gap| - (sum_j P (dP - delta)) (sum_j P |gap|)),
+// in fp32 from unrounded values: delta, which has the output's rounding in it, drops out.
 template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(SequenceArgs a, int blocks, bool vec) {
   constexpr int P = DP + pitch_pad<T>();
   __shared__ __attribute__((aligned(16))) T ks[kTile * P], vs[kTile * P];
   __shared__ int ids[kTile];
-  __shared__ float part[kTile];
   const Owner own = owner_of(blocks, a.H, blockIdx.x);
   const int b = own.b, h = own.h, hk = h / (a.H / a.Hk);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
@@ -334,9 +334,9 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
   const Scorer<T> score(a, h);
 
   f32x4 dq[DP / 16];
-  float far_dp, far, pdp;
+  float far, error, far_error;
   for (int strict = 0; strict < 2; ++strict) {
-    far_dp = far = pdp = 0.f;
+    far = error = far_error = 0.f;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) dq[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int first = 0; first * kTile < high; first += 64) {
@@ -364,13 +364,14 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
             float factor;
             const float x = score(a, s[kt][e], row.pos, key, factor);
             const float p = see ? exp2_of<T>(x - lse) : 0.f;
-            w[kt][e] = see ? p * (dp[kt][e] - delta) * factor : 0.f;
+            const float ds = see ? p * (dp[kt][e] - delta) : 0.f;
+            w[kt][e] = ds * factor;
             seen |= see ? 1u << (4 * kt + e) : 0u;
             if (a.slope_part && see) {
               const float gap = fabsf(float(row.pos - key));
-              pdp += p * dp[kt][e];
               far += p * gap;
-              far_dp += p * dp[kt][e] * gap;
+              error += ds;
+              far_error += ds * gap;
             }
           }
         add_transposed<T, DP>(ks, w, seen, strict != 0, false, dq);
@@ -394,15 +395,10 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
       }
   }
   if (a.slope_part) {
-    far_dp = column_sum(far_dp);
     far = column_sum(far);
-    pdp = column_sum(pdp);
-    if (grp == 0) part[wave * 16 + col] = valid ? -(far_dp - pdp * far) : 0.f;
-    __syncthreads();
-    if (tid < kTile) {
-      const float t = wave_sum(part[tid]);
-      if (tid == 0) a.slope_part[(int64_t(h) * a.B + b) * blocks + own.block] = t;
-    }
+    error = column_sum(error);
+    far_error = column_sum(far_error);
+    if (valid && grp == 0) a.slope_part[(int64_t(h) * a.B + b) * a.Nq + i] = -(far_error - error * far);
   }
 }
 
@@ -563,10 +559,11 @@ int sequence_ranges(const SequenceArgs &a, hipStream_t s) {
   return check_launch("sequence_attention");
 }
 
-int sequence_forward(const SequenceArgs &a, int dtype, hipStream_t s) {
+int sequence_forward(const SequenceArgs &a, int dtype, void *parts, int splits, hipStream_t s) {
   if (a.B == 0 || a.H == 0 || a.Nq == 0) return XFH_OK;
   XFH_TRY(check_grid(a));
   XFH_TRY(sequence_ranges(a, s));
+  if (dtype == XFH_BF16 && sequence_bf16_forward_fits(a)) return sequence_bf16_forward(a, parts, splits, s);
   const int d = std::max(a.D, a.Dv);
 #define XFH_SEQ_FORWARD(DP) return dtype == XFH_BF16 ? launch_forward<bf16, DP>(a, s) : launch_forward<float, DP>(a, s)
   if (d <= 32) XFH_SEQ_FORWARD(32);
@@ -576,7 +573,7 @@ int sequence_forward(const SequenceArgs &a, int dtype, hipStream_t s) {
 #undef XFH_SEQ_FORWARD
 }
 
-int64_t sequence_slope_part(int64_t B, int64_t H, int64_t Nq) { return H * B * ceil_div(Nq, int64_t(kTile)); }
+int64_t sequence_slope_part(int64_t B, int64_t H, int64_t Nq) { return H * B * Nq; }
 
 int sequence_backward(const SequenceArgs &a, int dtype, float *dslopes, hipStream_t s) {
   if (a.B > 0 && a.Hk > 0) {
@@ -585,7 +582,8 @@ int sequence_backward(const SequenceArgs &a, int dtype, float *dslopes, hipStrea
     const int d = std::max(a.D, a.Dv);
     int status = XFH_OK;
 #define XFH_SEQ_BACKWARD(DP) status = dtype == XFH_BF16 ? launch_backward<bf16, DP>(a, s) : launch_backward<float, DP>(a, s)
-    if (d <= 32) XFH_SEQ_BACKWARD(32);
+    if (dtype == XFH_BF16 && sequence_bf16_backward_fits(a)) status = sequence_bf16_backward(a, s);
+    else if (d <= 32) XFH_SEQ_BACKWARD(32);
     else if (d <= 64) XFH_SEQ_BACKWARD(64);
     else if (d <= 96) XFH_SEQ_BACKWARD(96);
     else XFH_SEQ_BACKWARD(128);
@@ -593,7 +591,7 @@ int sequence_backward(const SequenceArgs &a, int dtype, float *dslopes, hipStrea
     if (status != XFH_OK) return status;
   }
   if (!dslopes || a.H == 0) return XFH_OK;
-  dslopes_kernel<<<dim3(unsigned(a.H)), 256, 0, s>>>(a.slope_part, int64_t(a.B) * ceil_div(int64_t(a.Nq), int64_t(kTile)), dslopes);
+  dslopes_kernel<<<dim3(unsigned(a.H)), 256, 0, s>>>(a.slope_part, int64_t(a.B) * a.Nq, dslopes);
   return check_launch("sequence_attention_backward");
 }
 

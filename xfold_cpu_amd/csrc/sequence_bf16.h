@@ -1,0 +1,274 @@
+// Tiles of the bf16 sequence attention kernels (head dims that are multiples of 8, rows on 16 bytes).
+//
+// Products are 32x32x16 MFMAs with a wavefront's 32 owned tokens as columns: lane l = 32 half + c holds
+// column c, rows 8 (r / 4) + 4 half + r % 4 of a 32-row result (r = 0..15). For the next product, over
+// these rows, a step of 16 takes registers 8 s .. 8 s + 7 as they are: slot e < 4 of half h is row
+// 4 h + e, slot e >= 4 row 8 + 4 h + e - 4, and the other operand is read in the same order.
+//
+// A tile of 64 tokens lies row-major in LDS, DL elements a row, brought there by direct loads (a
+// wavefront writes 1 KB, lane i its bytes [16 i, 16 i + 16)). 16-byte chunk c of row r is at slot
+// c ^ 2 ((r / RPB) % PAIRS): the 8 rows that one cycle of a row-fragment read takes, and the 8 rows that
+// the transposing reads of a wavefront take, are then in different banks. What lies beyond a
+// matrix's end is a copy of its last row, beyond the head dim a copy of the row's first chunk: both
+// meet weights, or elements of the other operand, that are zero.
+#pragma once
+
+#include "sequence.h"
+
+namespace xfh {
+namespace seq {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((address_space(1))) void global_void;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// Head dims up to DL_ in LDS, KS_ steps of 16 in a product over the head dim, DT_ tiles of 32 of it in a result.
+template <int DL_, int KS_, int DT_> struct Dim {
+  static constexpr int DL = DL_, KS = KS_, DT = DT_;
+  static constexpr int RPB = 128 / DL, PAIRS = DL / 16;
+  static constexpr int ROW_PIECES = 512 / DL;            // rows of a 1 KB piece
+  static constexpr int PIECES = kTile / ROW_PIECES;      // pieces of a tile of 64
+  static_assert(DL == 32 || DL == 64 || DL == 128, "LDS rows of 64, 128 or 256 bytes");
+  static_assert(KS * 16 <= DL && DT * 32 <= DL, "products within the row");
+  static __device__ __forceinline__ int swizzle(int row) { return 2 * ((row / RPB) & (PAIRS - 1)); }
+};
+
+__device__ __forceinline__ f32x16 mfma32(const bf16x8 &a, const bf16x8 &b, const f32x16 &c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 zeros16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+// Row of register r of a 32-row result.
+__device__ __forceinline__ constexpr int row_of_register(int r) { return 8 * (r / 4) + r % 4; }   // + 4 half
+
+// Lane offsets (elements) into a tile.
+template <class D> struct Lane {
+  int half, col, rows, swz, tr[D::DT];
+  __device__ __forceinline__ Lane() {
+    const int lane = threadIdx.x & 63;
+    half = lane >> 5;
+    col = lane & 31;
+    rows = col * D::DL;
+    swz = D::swizzle(col);
+    // Transposing read: 16 lanes take 4 rows of 16 elements, 4 elements a lane.
+    const int i = lane & 15, row = 4 * half + i / 4, chunk = 2 * ((lane >> 4) & 1) + (i % 4) / 2;
+#pragma unroll
+    for (int t = 0; t < D::DT; ++t) tr[t] = row * D::DL + ((t * 4 + chunk) ^ D::swizzle(row)) * 8 + 4 * (i & 1);
+  }
+  // Rows 32 rt .. of a tile, elements 16 ks + 8 half ..: the A operand of a product over the head dim.
+  __device__ __forceinline__ bf16x8 row_fragment(const bf16 *tile, int rt, int ks) const {
+    return *reinterpret_cast<const bf16x8 *>(tile + rt * 32 * D::DL + rows + (((2 * ks) ^ swz) + half) * 8);
+  }
+  // Head dims 32 t .. as rows, 16 rows of the tile from 16 kk on as k: the A operand of a product over tokens.
+  __device__ __forceinline__ bf16x8 transposed(const bf16 *tile, int t, int kk) const {
+    const bf16 *p = tile + kk * 16 * D::DL + tr[t];
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 8 * D::DL));
+    const __attribute__((ext_vector_type(8))) short v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(bf16x8, v);
+  }
+  // [rows of the tile] x [owned columns] over the head dim.
+  __device__ __forceinline__ f32x16 product(const bf16 *tile, int rt, const bf16x8 (&own)[D::KS]) const {
+    f32x16 acc = zeros16();
+#pragma unroll
+    for (int ks = 0; ks < D::KS; ++ks) acc = mfma32(row_fragment(tile, rt, ks), own[ks], acc);
+    return acc;
+  }
+  // acc += tile^T w over the 16 rows from 16 kk on. STRICT: elements that are not finite are left
+  // out and added to the columns that see them (`seen`, 1 or 0): with SIGNS as what they are, else as NaN.
+  template <bool STRICT, bool SIGNS>
+  __device__ __forceinline__ void accumulate(const bf16 *tile, int kk, const bf16x8 &w, const bf16x8 &seen,
+                                             f32x16 (&acc)[D::DT]) const {
+#pragma unroll
+    for (int t = 0; t < D::DT; ++t) {
+      bf16x8 a = transposed(tile, t, kk);
+      if constexpr (STRICT) {
+        bf16x8 up, down;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = static_cast<float>(a[e]);
+          const bool bad = !(fabsf(x) < INFINITY);
+          up[e] = bf16(bad && !(SIGNS && x < 0.f) ? 1.f : 0.f);
+          down[e] = bf16(bad && !(SIGNS && x > 0.f) ? 1.f : 0.f);
+          if (bad) a[e] = bf16(0.f);
+        }
+        const f32x16 ups = mfma32(up, seen, zeros16()), downs = mfma32(down, seen, zeros16());
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (ups[r] > 0.f) acc[t][r] += INFINITY;
+          if (downs[r] > 0.f) acc[t][r] -= INFINITY;
+        }
+      }
+      acc[t] = mfma32(a, w, acc[t]);
+    }
+  }
+};
+
+// 8 registers of a result, rounded, as the B operand of a step of 16.
+__device__ __forceinline__ bf16x8 weights(const f32x16 &w, int first) {
+  bf16x8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = static_cast<bf16>(w[first + e]);
+  return v;
+}
+__device__ __forceinline__ bf16x8 weights_seen(uint32_t seen, int first) {
+  bf16x8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = bf16((seen >> (first + e)) & 1 ? 1.f : 0.f);
+  return v;
+}
+
+// The other lane of a column (the same column in the other half).
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// An owned token's row as B fragments (chunk 2 ks + half), zero beyond D.
+template <class D> __device__ __forceinline__ void own_row(bf16x8 (&f)[D::KS], const bf16 *row, int dim, bool valid, int half) {
+#pragma unroll
+  for (int ks = 0; ks < D::KS; ++ks) {
+    bf16x8 z = {};
+    const int at = ks * 16 + half * 8;
+    f[ks] = valid && at < dim ? *reinterpret_cast<const bf16x8 *>(row + at) : z;
+  }
+}
+
+// Direct loads of tiles of one matrix ([rows][dim], row stride in elements) by W wavefronts: piece j of
+// wavefront w is w + j W.
+template <class D, int W, int ROWS = kTile> struct Loader {
+  static constexpr int N = ROWS / D::ROW_PIECES / W;
+  static_assert(N * D::ROW_PIECES * W == ROWS, "whole pieces for each wavefront");
+  uint32_t offset[N];                                    // bytes from the tile's first row
+  const bf16 *base;
+  int64_t stride;
+  int wave, last, dim;                                   // last: the matrix's last row
+  __device__ __forceinline__ Loader(const bf16 *b, int64_t s, int rows, int d, int w)
+      : base(b), stride(s), wave(w), last(rows - 1), dim(d) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) offset[j] = uint32_t(int64_t(row(j)) * stride * 2) + chunk(j) * 16;
+  }
+  __device__ __forceinline__ int row(int j) const {
+    return (wave + j * W) * D::ROW_PIECES + int(threadIdx.x & 63) / (D::DL / 8);
+  }
+  __device__ __forceinline__ uint32_t chunk(int j) const {
+    const int c = int(threadIdx.x & 63) % (D::DL / 8) ^ D::swizzle(row(j));
+    return c * 8 < dim ? c : 0;
+  }
+  // Rows from `first` (at most the last one) on.
+  __device__ __forceinline__ void load(bf16 *tile, int first) const {
+    if (first + ROWS - 1 <= last) {
+      const char *p = reinterpret_cast<const char *>(base + int64_t(first) * stride);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        __builtin_amdgcn_global_load_lds((global_void *)(p + offset[j]), (lds_void *)(tile + (wave + j * W) * 512), 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const char *p = reinterpret_cast<const char *>(base + int64_t(min(first + row(j), last)) * stride) + chunk(j) * 16;
+        __builtin_amdgcn_global_load_lds((global_void *)p, (lds_void *)(tile + (wave + j * W) * 512), 16, 0, 0);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// How a score comes from a dot product: MODE bit 0 = cap, bit 1 = the general form without a cap (distance
+// slopes, or a scale that is not positive). Scores are in log 2 units; with MODE 0 what is held is the
+// dot product, and `unit` = scale log2 e goes into the exponent's multiply-add.
+template <int MODE> struct Score {
+  static constexpr bool CAP = MODE & 1, SLOPE = MODE & 2, RAW = MODE == 0;
+  float unit, to_exponent, cap2, slope;
+  __device__ __forceinline__ Score(const SequenceArgs &a, int h)
+      : unit(a.scale * kLog2e), to_exponent(CAP ? a.scale * 2.0f * kLog2e / a.cap : 0.f), cap2(a.cap * kLog2e),
+        slope(SLOPE && a.slopes ? a.slopes[h] * kLog2e : 0.f) {}
+  // gap = p_i - j; `bent` (1 - tanh^2) when asked for.
+  __device__ __forceinline__ float operator()(float dot, float gap, float *bent = nullptr) const {
+    float w = dot;
+    if constexpr (CAP) {
+      const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * to_exponent) + 1.0f);   // (1 - tanh) / 2
+      w = __builtin_fmaf(r, -2.0f * cap2, cap2);
+      if (bent) *bent = 4.0f * r * (1.0f - r);
+    } else if constexpr (SLOPE) {
+      w = dot * unit;
+    }
+    if constexpr (SLOPE) w = __builtin_fmaf(-slope, fabsf(gap), w);
+    return w;
+  }
+  // exp2(score - m)
+  __device__ __forceinline__ float weight(float w, float m) const {
+    return __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(w, unit, -m) : w - m);
+  }
+  __device__ __forceinline__ float in_log2(float w) const { return RAW ? w * unit : w; }
+};
+
+// A tile of a walk: its number (-1: none is left), whether this wavefront's columns see any and all of it.
+struct Step { int tile; bool mine, whole; };
+
+// The walk over tiles [first, end), 64 of them at a time, one per lane. test(tile) says which of {the
+// workgroup needs it, the wavefront needs it, the wavefront's columns see it whole} hold.
+struct Needs { bool block, mine, whole; };
+struct Walk {
+  int first, end;
+  uint64_t need = 0, mine = 0, whole = 0;
+  __device__ __forceinline__ Walk(int f, int e) : first(f - 64), end(e) {}
+  template <class F> __device__ __forceinline__ Step next(F test) {
+    while (!need) {
+      first += 64;
+      if (first >= end) return {-1, false, false};
+      const int tile = first + int(threadIdx.x & 63);
+      Needs n{false, false, false};
+      if (tile < end) n = test(tile);
+      need = __ballot(n.block);
+      mine = __ballot(n.block && n.mine);
+      whole = __ballot(n.block && n.mine && n.whole);
+    }
+    const int bit = __builtin_ctzll(need);
+    need &= need - 1;
+    return {first + bit, bool((mine >> bit) & 1), bool((whole >> bit) & 1)};
+  }
+};
+
+// Bounds and documents of the keys that a run of queries sees.
+struct Span { int low, high; Range range; };
+__device__ __forceinline__ Span span_of(const SequenceArgs &a, const Place &p, int b, int i0, int i1) {
+  Span s{0, 0, Range{0x7fffffff, -1, 0, 0}};
+  if (i0 > i1) return s;
+  s.low = limit_of(a, p, i0);
+  s.high = limit_of(a, p, i1);
+  if (a.documents) s.range = query_range(a, p, b, i0, i1);
+  return s;
+}
+__device__ __forceinline__ Needs key_tile_needs(const SequenceArgs &a, int b, int tile, const Span &block, const Span &wave) {
+  const int k0 = tile * kTile;
+  Needs n{k0 < block.high, k0 < wave.high, k0 + kTile <= wave.low};
+  if (a.documents && n.block) {
+    const Range r = static_cast<const Range *>(a.ranges)[int64_t(b) * a.tiles + tile];
+    n.block = overlap(r, block.range);
+    n.mine = n.mine && overlap(r, wave.range);
+    n.whole = n.whole && same_document(r, wave.range);
+  }
+  return n;
+}
+
+// Scores of hidden pairs in a result of 32 rows (keys k0 ..) become -infinity; returns the bits of the seen.
+__device__ __forceinline__ uint32_t hide_keys(const SequenceArgs &a, int b, int k0, int half, const Row &row, f32x16 &w) {
+  uint32_t seen = 0;
+  const int limit = row.limit - k0 - 4 * half;
+  const int32_t *ids = a.documents ? a.documents + int64_t(b) * a.documents_stride + k0 + 4 * half : nullptr;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    bool see = row_of_register(r) < limit;
+    if (ids && see) see = ids[row_of_register(r)] == row.document;
+    w[r] = see ? w[r] : -INFINITY;
+    seen |= see ? 1u << r : 0u;
+  }
+  return seen;
+}
+
+}  // namespace seq
+}  // namespace xfh
