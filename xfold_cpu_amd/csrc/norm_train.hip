@@ -295,27 +295,33 @@ template <typename T, typename TO> __global__ __launch_bounds__(kThreads) void n
   a.partial[(int64_t(gridDim.y) + blockIdx.y) * a.C + c] = db;
 }
 
-// out[which][c] = sum over the blocks' partial sums: 16 columns by 16 slices of blocks per workgroup,
-// every sum in the blocks' order.
-__global__ __launch_bounds__(kThreads) void norm_params_kernel(const float *partial, int blocks, int C, void *dw,
-                                                               int dw_dtype, void *db, int db_dtype) {
-  __shared__ float part[16][17];
+// out[which][c] = sum over the blocks' partial sums: 16 columns by 64 slices of blocks per workgroup (each
+// slice 4 sums in flight), every sum in a fixed order.
+constexpr int kSlices = 64;
+__global__ __launch_bounds__(16 * kSlices) void norm_params_kernel(const float *partial, int blocks, int C, void *dw,
+                                                                   int dw_dtype, void *db, int db_dtype) {
+  __shared__ float part[kSlices][17];
   void *out = blockIdx.y ? db : dw;
   if (!out) return;
   const int dtype = blockIdx.y ? db_dtype : dw_dtype;
   const int col = threadIdx.x & 15, slice = threadIdx.x >> 4, c = int(blockIdx.x) * 16 + col;
   const float *p = partial + int64_t(blockIdx.y) * blocks * C + c;
-  float t = 0.f;
-  if (c < C)
-    for (int r = slice; r < blocks; r += 16) t += p[int64_t(r) * C];
-  part[slice][col] = t;
-  __syncthreads();
-  if (slice == 0 && c < C) {
-    t = 0.f;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < C) {
+    int r = slice;
+    for (; r + 3 * kSlices < blocks; r += 4 * kSlices)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) t += part[r][col];
-    if (dtype == XFH_F32) static_cast<float *>(out)[c] = t;
-    else static_cast<bf16 *>(out)[c] = bf16(t);
+      for (int u = 0; u < 4; ++u) t[u] += p[int64_t(r + u * kSlices) * C];
+    for (; r < blocks; r += kSlices) t[0] += p[int64_t(r) * C];
+  }
+  part[slice][col] = (t[0] + t[1]) + (t[2] + t[3]);
+  for (int n = kSlices / 2; n > 0; n /= 2) {
+    __syncthreads();
+    if (slice < n) part[slice][col] += part[slice + n][col];
+  }
+  if (slice == 0 && c < C) {
+    if (dtype == XFH_F32) static_cast<float *>(out)[c] = part[0][col];
+    else static_cast<bf16 *>(out)[c] = bf16(part[0][col]);
   }
 }
 
@@ -410,7 +416,7 @@ int norm_train_backward(const void *dy, int dy_dtype, int64_t lddy, const void *
   if (rows > 0 && (dx || a.partial)) XFH_TRY(launch_norm(a, x_dtype, dy_dtype, true, s));
   if (!dw && !db) return XFH_OK;
   const int64_t blocks = backward_blocks(rows, cols);    // no rows: sums of nothing, zeros
-  norm_params_kernel<<<dim3(unsigned(ceil_div(cols, int64_t(16))), 2), kThreads, 0, s>>>(partial, int(blocks), int(cols), dw,
+  norm_params_kernel<<<dim3(unsigned(ceil_div(cols, int64_t(16))), 2), 16 * kSlices, 0, s>>>(partial, int(blocks), int(cols), dw,
                                                                                        dw_dtype, db, db_dtype);
   return check_launch("layer_norm_backward");
 }

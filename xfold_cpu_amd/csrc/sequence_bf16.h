@@ -255,17 +255,38 @@ __device__ __forceinline__ Needs key_tile_needs(const SequenceArgs &a, int b, in
   return n;
 }
 
-// Scores of hidden pairs in a result of 32 rows (keys k0 ..) become -infinity; returns the bits of the seen.
-__device__ __forceinline__ uint32_t hide_keys(const SequenceArgs &a, int b, int k0, int half, const Row &row, f32x16 &w) {
+// What a wavefront looks up to hide pairs: bounds and documents of the rows of a tile, in LDS of its own (a
+// lane works out one row; the 16 rows of a lane's registers are then eight 16-byte reads).
+struct Marks { int limit[kTile], document[kTile]; };
+__device__ __forceinline__ void marks_written() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+// Documents of the keys of a tile (k0 ..; beyond n they stay what they were, and are not looked at).
+__device__ __forceinline__ void mark_keys(const SequenceArgs &a, int b, int k0, int n, Marks &marks) {
+  if (!a.documents) return;
+  const int key = k0 + int(threadIdx.x & 63);
+  marks_written();                                       // (the tile before is done with them)
+  if (key < n) marks.document[threadIdx.x & 63] = a.documents[int64_t(b) * a.documents_stride + key];
+  marks_written();
+}
+// Scores of hidden pairs in rows 32 rt .. of a tile of keys (k0 ..) become -infinity; returns the bits of the seen.
+__device__ __forceinline__ uint32_t hide_keys(const SequenceArgs &a, const Marks &marks, int rt, int k0, int half,
+                                              const Row &row, f32x16 &w) {
   uint32_t seen = 0;
-  const int limit = row.limit - k0 - 4 * half;
-  const int32_t *ids = a.documents ? a.documents + int64_t(b) * a.documents_stride + k0 + 4 * half : nullptr;
+  const int limit = row.limit - k0 - rt * 32 - 4 * half;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    bool see = row_of_register(r) < limit;
-    if (ids && see) see = ids[row_of_register(r)] == row.document;
-    w[r] = see ? w[r] : -INFINITY;
-    seen |= see ? 1u << r : 0u;
+  for (int j = 0; j < 4; ++j) {
+    int4 ids{row.document, row.document, row.document, row.document};
+    if (a.documents) ids = *reinterpret_cast<const int4 *>(marks.document + rt * 32 + 8 * j + 4 * half);
+    const int id[4] = {ids.x, ids.y, ids.z, ids.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool see = (8 * j + e < limit) & (id[e] == row.document);
+      w[4 * j + e] = see ? w[4 * j + e] : -INFINITY;
+      seen |= see ? 1u << (4 * j + e) : 0u;
+    }
   }
   return seen;
 }

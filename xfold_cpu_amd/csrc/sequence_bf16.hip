@@ -3,7 +3,8 @@
 // Forward and dq: the columns of a workgroup are 128 queries of the heads that share a key head, query by
 // query (column c = query c / G, head c % G of the group of G): the heads of one query read the same
 // keys, and a few queries fill a tile. A wavefront owns 32 of them, with K and V tiles shared.
-// dk and dv: the columns are 128 keys; the loop goes over the heads of the group and their queries.
+// dk and dv: the columns are 64 keys, each 32 of them with two wavefronts that take turns at the queries (half
+// a tile each); the loop goes over the heads of the group and their queries.
 //
 // Tiles are brought to LDS by direct loads, one ahead of the one in use (two stages, one barrier a tile).
 #include <algorithm>
@@ -25,12 +26,14 @@ constexpr float kLowest = -3.402823466e38f;              // running maximum befo
 // raised (and o and l scaled) only when a score exceeds it by kSlack, so weights are at most 2^kSlack.
 template <class D, int MODE, bool STRICT, int ROWS>
 __device__ __forceinline__ void forward_tile(const SequenceArgs &a, const Lane<D> &ln, const bf16 *kt, const bf16 *vt,
-                                             const bf16x8 (&qf)[D::KS], const Score<MODE> &score, int b, int k0, bool whole,
-                                             const Row &row, float &m, float &l, f32x16 (&o)[D::DT]) {
+                                             const bf16x8 (&qf)[D::KS], const Score<MODE> &score, int b, int k0, int n,
+                                             bool whole, const Row &row, Marks &marks, float &m, float &l,
+                                             f32x16 (&o)[D::DT]) {
   constexpr int RT = ROWS / 32;
   f32x16 w[RT];
   uint32_t seen[RT];
   float top = kLowest;
+  if (!whole) mark_keys(a, b, k0, n, marks);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) w[rt] = ln.product(kt, rt, qf);
 #pragma unroll
@@ -41,7 +44,7 @@ __device__ __forceinline__ void forward_tile(const SequenceArgs &a, const Lane<D
       for (int r = 0; r < 16; ++r) w[rt][r] = score(w[rt][r], gap - float(row_of_register(r)));
     }
     seen[rt] = 0xffff;
-    if (!whole) seen[rt] = hide_keys(a, b, k0 + rt * 32, ln.half, row, w[rt]);
+    if (!whole) seen[rt] = hide_keys(a, marks, rt, k0, ln.half, row, w[rt]);
 #pragma unroll
     for (int r = 0; r < 16; ++r) top = fmaxf(top, w[rt][r]);
   }
@@ -103,8 +106,8 @@ struct Parts {
 template <class D, int MODE, bool STRICT>
 __device__ __forceinline__ void forward_walk(const SequenceArgs &a, const Lane<D> &ln, bf16 *lds, const Loader<D, 4> &kl,
                                              const Loader<D, 4> &vl, const bf16x8 (&qf)[D::KS], const Score<MODE> &score,
-                                             int b, int first, int end, const Span &block, const Span &wave, const Row &row,
-                                             float &m, float &l, f32x16 (&o)[D::DT]) {
+                                             int b, int first, int end, int n, const Span &block, const Span &wave,
+                                             const Row &row, Marks &marks, float &m, float &l, f32x16 (&o)[D::DT]) {
   constexpr int TILE = kTile * D::DL;
   m = kLowest;
   l = 0.f;
@@ -129,7 +132,7 @@ __device__ __forceinline__ void forward_walk(const SequenceArgs &a, const Lane<D
     }
     if (now.mine) {
       const bf16 *kt = lds + stage * 2 * TILE;
-      forward_tile<D, MODE, STRICT, kTile>(a, ln, kt, kt + TILE, qf, score, b, now.tile * kTile, now.whole, row, m, l, o);
+      forward_tile<D, MODE, STRICT, kTile>(a, ln, kt, kt + TILE, qf, score, b, now.tile * kTile, n, now.whole, row, marks, m, l, o);
     }
     now = then;
     stage ^= 1;
@@ -140,6 +143,7 @@ template <class D, int MODE>
 __global__ __launch_bounds__(256, 2) void forward_bf16_kernel(SequenceArgs a, int blocks, Parts parts) {
   constexpr int TILE = kTile * D::DL;
   __shared__ __attribute__((aligned(1024))) bf16 lds[4 * TILE];
+  __shared__ __attribute__((aligned(16))) Marks marks[4];
   const int group = a.H / a.Hk, columns = group * a.Nq;
   const int hk = blockIdx.x % a.Hk;
   int rest = blockIdx.x / a.Hk;
@@ -170,9 +174,9 @@ __global__ __launch_bounds__(256, 2) void forward_bf16_kernel(SequenceArgs a, in
   }
   f32x16 o[D::DT];
   float m, l;
-  forward_walk<D, MODE, false>(a, ln, lds, kl, vl, qf, score, b, first, end, block, mine, row, m, l, o);
+  forward_walk<D, MODE, false>(a, ln, lds, kl, vl, qf, score, b, first, end, place.n, block, mine, row, marks[wave], m, l, o);
   if (__syncthreads_or(valid && any_bad<D>(o)))
-    forward_walk<D, MODE, true>(a, ln, lds, kl, vl, qf, score, b, first, end, block, mine, row, m, l, o);
+    forward_walk<D, MODE, true>(a, ln, lds, kl, vl, qf, score, b, first, end, place.n, block, mine, row, marks[wave], m, l, o);
   l += other_half(l);
   if (!valid) return;
   if (parts.splits > 1) {
@@ -198,8 +202,8 @@ __global__ __launch_bounds__(256, 2) void forward_bf16_kernel(SequenceArgs a, in
 template <class D, int MODE, bool STRICT>
 __device__ __forceinline__ void token_walk(const SequenceArgs &a, const Lane<D> &ln, bf16 *lds, const Loader<D, 1, 32> &kl,
                                            const Loader<D, 1, 32> &vl, const bf16x8 (&qf)[D::KS], const Score<MODE> &score,
-                                           int b, int first, int end, const Span &span, const Row &row, float &m, float &l,
-                                           f32x16 (&o)[D::DT]) {
+                                           int b, int first, int end, int n, const Span &span, const Row &row, Marks &marks,
+                                           float &m, float &l, f32x16 (&o)[D::DT]) {
   constexpr int TILE = 32 * D::DL;
   m = kLowest;
   l = 0.f;
@@ -224,7 +228,7 @@ __device__ __forceinline__ void token_walk(const SequenceArgs &a, const Lane<D> 
       whole = whole && same_document(r, span.range);
     }
     const bf16 *kt = lds + stage * 2 * TILE;
-    if (need) forward_tile<D, MODE, STRICT, 32>(a, ln, kt, kt + TILE, qf, score, b, tile * 32, whole, row, m, l, o);
+    if (need) forward_tile<D, MODE, STRICT, 32>(a, ln, kt, kt + TILE, qf, score, b, tile * 32, n, whole, row, marks, m, l, o);
     // The loads of the step after next go to this stage: every read of it has to be done.
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     stage ^= 1;
@@ -235,6 +239,7 @@ template <class D, int MODE>
 __global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, int blocks, Parts parts) {
   constexpr int TILE = 32 * D::DL, PITCH = D::DT * 32 + 4;
   __shared__ __attribute__((aligned(1024))) bf16 lds[4][4 * TILE];
+  __shared__ __attribute__((aligned(16))) Marks marks[4];
   __shared__ float2 ml[4][32];
   static_assert(sizeof(lds) >= 4 * 32 * PITCH * 4 || D::DL < 128, "joined in the tiles' memory");
   __shared__ float joined[D::DL < 128 ? 4 * 32 * PITCH : 1];
@@ -260,9 +265,9 @@ __global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, int 
   const int first = min(split * per, tiles), end = min(first + per, tiles);
   f32x16 o[D::DT];
   float m, l;
-  token_walk<D, MODE, false>(a, ln, lds[wave], kl, vl, qf, score, b, first + wave, end, span, row, m, l, o);
+  token_walk<D, MODE, false>(a, ln, lds[wave], kl, vl, qf, score, b, first + wave, end, place.n, span, row, marks[wave], m, l, o);
   if (__syncthreads_or(valid && any_bad<D>(o)))
-    token_walk<D, MODE, true>(a, ln, lds[wave], kl, vl, qf, score, b, first + wave, end, span, row, m, l, o);
+    token_walk<D, MODE, true>(a, ln, lds[wave], kl, vl, qf, score, b, first + wave, end, place.n, span, row, marks[wave], m, l, o);
   l += other_half(l);
   __syncthreads();
   if (ln.half == 0) ml[wave][c] = make_float2(m, l);
@@ -297,25 +302,31 @@ __global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, int 
   }
 }
 
-// Joins the parts of split keys, in their order: a thread per element.
+// Joins the parts of split keys, in their order: a thread per 4 elements (Dv is a multiple of 8 here).
 __global__ __launch_bounds__(256) void join_kernel(SequenceArgs a, Parts parts) {
-  const int group = a.H / a.Hk, columns = group * a.Nq;
+  const int group = a.H / a.Hk, columns = group * a.Nq, quads = a.Dv / 4;
   const int64_t total = int64_t(a.B) * a.Hk * columns, at = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= total * a.Dv) return;
-  const int64_t column = at / a.Dv;
-  const int d = int(at % a.Dv);
+  if (at >= total * quads) return;
+  const int64_t column = at / quads;
+  const int d = int(at - column * quads) * 4;
   float top = kLowest;
   for (int s = 0; s < parts.splits; ++s) top = fmaxf(top, parts.ml[s * total + column].x);
-  float sum = 0.f, value = 0.f;
+  float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < parts.splits; ++s) {
     const float2 p = parts.ml[s * total + column];
+    const float4 o = *reinterpret_cast<const float4 *>(parts.o + (s * total + column) * a.Dv + d);
     const float f = __builtin_amdgcn_exp2f(p.x - top);
     sum += f * p.y;
-    value += f * parts.o[(s * total + column) * a.Dv + d];
+    v[0] += f * o.x; v[1] += f * o.y; v[2] += f * o.z; v[3] += f * o.w;
   }
-  const int c = int(column % columns), hk = int(column / columns % a.Hk), b = int(column / columns / a.Hk);
+  const int c = int(column % columns), bk = int(column / columns), hk = bk % a.Hk, b = bk / a.Hk;
   const int i = c / group, h = hk * group + c % group;
-  static_cast<bf16 *>(a.out)[b * a.os[0] + h * a.os[1] + i * a.os[2] + d] = bf16(sum == 0.f ? 0.f : value / sum);
+  bf16 *out = static_cast<bf16 *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2] + d;
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  bf16x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = static_cast<bf16>(v[e] * inv);
+  *reinterpret_cast<bf16x4 *>(out) = r;
   if (a.lse && d == 0) a.lse[(int64_t(b) * a.H + h) * a.Nq + i] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
@@ -326,8 +337,9 @@ struct SlopeSums { float far, error, far_error; };       // sum P |gap|, sum P (
 template <class D, int MODE, bool STRICT>
 __device__ __forceinline__ void dq_walk(const SequenceArgs &a, const Lane<D> &ln, bf16 *lds, const Loader<D, 4> &kl,
                                         const Loader<D, 4> &vl, const bf16x8 (&qf)[D::KS], const bf16x8 (&gf)[D::KS],
-                                        const Score<MODE> &score, int b, int end, const Span &block, const Span &wave,
-                                        const Row &row, float lse, float delta, f32x16 (&dq)[D::DT], SlopeSums &sums) {
+                                        const Score<MODE> &score, int b, int end, int n, const Span &block,
+                                        const Span &wave, const Row &row, Marks &marks, float lse, float delta,
+                                        f32x16 (&dq)[D::DT], SlopeSums &sums) {
   constexpr int TILE = kTile * D::DL;
   sums = SlopeSums{0.f, 0.f, 0.f};
 #pragma unroll
@@ -351,6 +363,7 @@ __device__ __forceinline__ void dq_walk(const SequenceArgs &a, const Lane<D> &ln
     }
     if (now.mine) {
       const bf16 *kt = lds + stage * 2 * TILE, *vt = kt + TILE;
+      if (!now.whole) mark_keys(a, b, now.tile * kTile, n, marks);
 #pragma unroll
       for (int rt = 0; rt < 2; ++rt) {
         const int k0 = now.tile * kTile + rt * 32;
@@ -363,7 +376,7 @@ __device__ __forceinline__ void dq_walk(const SequenceArgs &a, const Lane<D> &ln
           if constexpr (Score<MODE>::CAP) bent[r] = f;
         }
         uint32_t seen = 0xffff;
-        if (!now.whole) seen = hide_keys(a, b, k0, ln.half, row, w);
+        if (!now.whole) seen = hide_keys(a, marks, rt, now.tile * kTile, ln.half, row, w);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float p = score.weight(w[r], lse), error = dp[r] - delta;
@@ -394,6 +407,7 @@ template <class D, int MODE>
 __global__ __launch_bounds__(256, 2) void dq_bf16_kernel(SequenceArgs a, int blocks) {
   constexpr int TILE = kTile * D::DL;
   __shared__ __attribute__((aligned(1024))) bf16 lds[4 * TILE];
+  __shared__ __attribute__((aligned(16))) Marks marks[4];
   const int group = a.H / a.Hk, columns = group * a.Nq;
   const int hk = blockIdx.x % a.Hk, rest = blockIdx.x / a.Hk, blk = blocks - 1 - rest % blocks, b = rest / blocks;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -429,9 +443,9 @@ __global__ __launch_bounds__(256, 2) void dq_bf16_kernel(SequenceArgs a, int blo
   const int end = (block.high + kTile - 1) / kTile;
   f32x16 dq[D::DT];
   SlopeSums sums;
-  dq_walk<D, MODE, false>(a, ln, lds, kl, vl, qf, gf, score, b, end, block, mine, row, lse, delta, dq, sums);
+  dq_walk<D, MODE, false>(a, ln, lds, kl, vl, qf, gf, score, b, end, place.n, block, mine, row, marks[wave], lse, delta, dq, sums);
   if (__syncthreads_or(valid && any_bad<D>(dq)))
-    dq_walk<D, MODE, true>(a, ln, lds, kl, vl, qf, gf, score, b, end, block, mine, row, lse, delta, dq, sums);
+    dq_walk<D, MODE, true>(a, ln, lds, kl, vl, qf, gf, score, b, end, place.n, block, mine, row, marks[wave], lse, delta, dq, sums);
   if (valid)
     store_column<D>(static_cast<bf16 *>(a.dq) + b * a.dqs[0] + h * a.dqs[1] + i * a.dqs[2], a.D, dq, a.scale, ln.half);
   if constexpr (Score<MODE>::SLOPE) {
@@ -446,24 +460,40 @@ __global__ __launch_bounds__(256, 2) void dq_bf16_kernel(SequenceArgs a, int blo
 
 // ------------------------------------------------------------------------------ dk, dv
 
-// Scores of hidden pairs in 32 rows (queries i0 ..) of one key column become -infinity.
-__device__ __forceinline__ uint32_t hide_queries(const SequenceArgs &a, const Place &place, int b, int i0, int half, int key,
-                                                 int document, f32x16 &w) {
+// Bounds and documents of 32 queries (i0 ..), a lane each.
+__device__ __forceinline__ void mark_queries(const SequenceArgs &a, const Place &place, int b, int i0, Marks &marks) {
+  const int at = threadIdx.x & 31;
+  const Row row = row_of(a, place, b, i0 + at);
+  marks_written();                                       // (the tile before is done with them)
+  marks.limit[at] = row.limit;
+  marks.document[at] = row.document;
+  marks_written();
+}
+// Scores of hidden pairs of one key column become -infinity.
+__device__ __forceinline__ uint32_t hide_queries(const Marks &marks, int half, int key, int document, f32x16 &w) {
   uint32_t seen = 0;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const Row row = row_of(a, place, b, i0 + 4 * half + row_of_register(r));
-    const bool see = key < row.limit && (!a.documents || row.document == document);
-    w[r] = see ? w[r] : -INFINITY;
-    seen |= see ? 1u << r : 0u;
+  for (int j = 0; j < 4; ++j) {
+    const int4 limits = *reinterpret_cast<const int4 *>(marks.limit + 8 * j + 4 * half);
+    const int4 ids = *reinterpret_cast<const int4 *>(marks.document + 8 * j + 4 * half);
+    const int limit[4] = {limits.x, limits.y, limits.z, limits.w}, id[4] = {ids.x, ids.y, ids.z, ids.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool see = (key < limit[e]) & (id[e] == document);
+      w[4 * j + e] = see ? w[4 * j + e] : -INFINITY;
+      seen |= see ? 1u << (4 * j + e) : 0u;
+    }
   }
   return seen;
 }
 
+constexpr int kKeys = 64;                                // keys of a workgroup: 2 groups of 32, each with 2 wavefronts
+
+// One wavefront: 32 keys from kw on, and of each tile of 64 queries the 32 from 32 rt on.
 template <class D, int MODE, bool STRICT>
-__device__ __forceinline__ void dkv_walk(const SequenceArgs &a, const Lane<D> &ln, bf16 *lds, float *stats,
+__device__ __forceinline__ void dkv_walk(const SequenceArgs &a, const Lane<D> &ln, bf16 *lds, float *stats, Marks &marks,
                                          const bf16x8 (&kf)[D::KS], const bf16x8 (&vf)[D::KS], int b, int hk, int wave, int kb,
-                                         int kw, int key, int document, const Place &place, f32x16 (&dk)[D::DT],
+                                         int kw, int rt, int key, int document, const Place &place, f32x16 (&dk)[D::DT],
                                          f32x16 (&dv)[D::DT]) {
   constexpr int TILE = kTile * D::DL;
   const int group = a.H / a.Hk, qtiles = (a.Nq + kTile - 1) / kTile;
@@ -472,22 +502,16 @@ __device__ __forceinline__ void dkv_walk(const SequenceArgs &a, const Lane<D> &l
     dk[t] = zeros16();
     dv[t] = zeros16();
   }
-  const Range none{0x7fffffff, -1, 0, 0};
-  Range block_range = none, wave_range = none;
-  if (a.documents) {
-    const Range *r = static_cast<const Range *>(a.ranges) + int64_t(b) * a.tiles;
-    const int t0 = kb / kTile, t1 = min(t0 + 1, a.tiles - 1);
-    block_range = Range{min(r[t0].x, r[t1].x), max(r[t0].y, r[t1].y), 0, 0};
-    if (kw < a.Nk) wave_range = r[kw / kTile];
-  }
+  Range range{0x7fffffff, -1, 0, 0};
+  if (a.documents) range = static_cast<const Range *>(a.ranges)[int64_t(b) * a.tiles + kb / kTile];
   const auto test = [&](int tile) {
-    const int i0 = tile * kTile, i1 = min(i0 + kTile, a.Nq) - 1, high = limit_of(a, place, i1);
-    Needs n{high > kb, high > kw, i0 + kTile <= a.Nq && limit_of(a, place, i0) >= kw + 32};
+    const int i0 = tile * kTile + rt * 32, i1 = min(i0 + 32, a.Nq) - 1, last = min(tile * kTile + kTile, a.Nq) - 1;
+    Needs n{limit_of(a, place, last) > kb, i0 <= i1 && limit_of(a, place, max(i1, 0)) > kw,
+            i0 + 32 <= a.Nq && limit_of(a, place, i0) >= kw + 32};
     if (a.documents && n.block) {
-      const Range r = query_range(a, place, b, i0, i1);
-      n.block = overlap(r, block_range);
-      n.mine = n.mine && overlap(r, wave_range);
-      n.whole = n.whole && same_document(r, wave_range);
+      const Range r = query_range(a, place, b, tile * kTile, last);
+      n.block = overlap(r, range);
+      n.whole = n.whole && same_document(r, range);
     }
     return n;
   };
@@ -518,41 +542,39 @@ __device__ __forceinline__ void dkv_walk(const SequenceArgs &a, const Lane<D> &l
       if (then.tile >= 0) load(then.tile, stage ^ 1);
       if (now.mine) {
         const bf16 *qt = lds + stage * 2 * TILE, *gt = qt + TILE;
-        const float *lses = stats + stage * 2 * kTile, *deltas = lses + kTile;
+        const float *lses = stats + stage * 2 * kTile + rt * 32, *deltas = lses + kTile;
+        const int i0 = now.tile * kTile + rt * 32;
+        if (!now.whole) mark_queries(a, place, b, i0, marks);
+        f32x16 w = ln.product(qt, rt, kf), dp = ln.product(gt, rt, vf), bent;
+        const float gap = float(i0 + place.shift + 4 * ln.half - key);
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
-          const int i0 = now.tile * kTile + rt * 32;
-          f32x16 w = ln.product(qt, rt, kf), dp = ln.product(gt, rt, vf), bent;
-          const float gap = float(i0 + place.shift + 4 * ln.half - key);
+        for (int r = 0; r < 16; ++r) {
+          float f = 1.f;
+          w[r] = score(w[r], gap + float(row_of_register(r)), &f);
+          if constexpr (Score<MODE>::CAP) bent[r] = f;
+        }
+        uint32_t seen = 0xffff;
+        if (!now.whole) seen = hide_queries(marks, ln.half, key, document, w);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            float f = 1.f;
-            w[r] = score(w[r], gap + float(row_of_register(r)), &f);
-            if constexpr (Score<MODE>::CAP) bent[r] = f;
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 lse = *reinterpret_cast<const f32x4 *>(lses + 8 * j + 4 * ln.half);
+          const f32x4 delta = *reinterpret_cast<const f32x4 *>(deltas + 8 * j + 4 * ln.half);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * j + e;
+            const bool see = now.whole || ((seen >> r) & 1);
+            const float p = see ? score.weight(w[r], lse[e]) : 0.f;
+            float ds = see ? p * (dp[r] - delta[e]) : 0.f;
+            if constexpr (Score<MODE>::CAP) ds *= bent[r];
+            w[r] = p;
+            dp[r] = ds;
           }
-          uint32_t seen = 0xffff;
-          if (!now.whole) seen = hide_queries(a, place, b, i0, ln.half, key, document, w);
+        }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const f32x4 lse = *reinterpret_cast<const f32x4 *>(lses + rt * 32 + 8 * j + 4 * ln.half);
-            const f32x4 delta = *reinterpret_cast<const f32x4 *>(deltas + rt * 32 + 8 * j + 4 * ln.half);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = 4 * j + e;
-              const bool see = now.whole || ((seen >> r) & 1);
-              const float p = see ? score.weight(w[r], lse[e]) : 0.f;
-              float ds = see ? p * (dp[r] - delta[e]) : 0.f;
-              if constexpr (Score<MODE>::CAP) ds *= bent[r];
-              w[r] = p;
-              dp[r] = ds;
-            }
-          }
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const bf16x8 sf = weights_seen(seen, 8 * s);
-            ln.template accumulate<STRICT, false>(gt, 2 * rt + s, weights(w, 8 * s), sf, dv);
-            ln.template accumulate<STRICT, false>(qt, 2 * rt + s, weights(dp, 8 * s), sf, dk);
-          }
+        for (int s = 0; s < 2; ++s) {
+          const bf16x8 sf = weights_seen(seen, 8 * s);
+          ln.template accumulate<STRICT, false>(gt, 2 * rt + s, weights(w, 8 * s), sf, dv);
+          ln.template accumulate<STRICT, false>(qt, 2 * rt + s, weights(dp, 8 * s), sf, dk);
         }
       }
       now = then;
@@ -562,32 +584,48 @@ __device__ __forceinline__ void dkv_walk(const SequenceArgs &a, const Lane<D> &l
 }
 
 template <class D, int MODE>
-__global__ __launch_bounds__(256, D::DL == 128 ? 1 : 2) void dkv_bf16_kernel(SequenceArgs a, int blocks) {
-  constexpr int TILE = kTile * D::DL;
-  __shared__ __attribute__((aligned(1024))) bf16 lds[4 * TILE];
+__global__ __launch_bounds__(256, 2) void dkv_bf16_kernel(SequenceArgs a, int blocks) {
+  constexpr int TILE = kTile * D::DL, JOIN = 2 * 2 * D::DT * 16 * 64;   // floats: 2 key groups, dk and dv
+  __shared__ __attribute__((aligned(1024))) unsigned char memory[JOIN * 4 > 8 * TILE ? JOIN * 4 : 8 * TILE];
   __shared__ __attribute__((aligned(1024))) float stats[4 * kTile];
+  __shared__ __attribute__((aligned(16))) Marks marks[4];
+  bf16 *lds = reinterpret_cast<bf16 *>(memory);
   const int hk = blockIdx.x % a.Hk, rest = blockIdx.x / a.Hk, blk = rest % blocks, b = rest / blocks;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rt = wave >> 1;
   const Lane<D> ln;
   const Place place = place_of(a, b);
-  const int kb = blk * kColumns, kw = kb + wave * 32, key = kw + ln.col;
+  const int kb = blk * kKeys, kw = kb + (wave & 1) * 32, key = kw + ln.col;
   const bool valid = key < place.n;
   bf16x8 kf[D::KS], vf[D::KS];
   own_row<D>(kf, static_cast<const bf16 *>(a.k) + b * a.ks[0] + hk * a.ks[1] + key * a.ks[2], a.D, valid, ln.half);
   own_row<D>(vf, static_cast<const bf16 *>(a.v) + b * a.vs[0] + hk * a.vs[1] + key * a.vs[2], a.Dv, valid, ln.half);
-  const int document = a.documents && valid ? a.documents[int64_t(b) * a.documents_stride + key] : -1;
+  int document = 0;                                      // (as row_of has it without documents)
+  if (a.documents) document = valid ? a.documents[int64_t(b) * a.documents_stride + key] : -1;
   f32x16 dk[D::DT], dv[D::DT];
-  dkv_walk<D, MODE, false>(a, ln, lds, stats, kf, vf, b, hk, wave, kb, kw, key, document, place, dk, dv);
+  dkv_walk<D, MODE, false>(a, ln, lds, stats, marks[wave], kf, vf, b, hk, wave, kb, kw, rt, key, document, place, dk, dv);
   if (__syncthreads_or(valid && (any_bad<D>(dk) || any_bad<D>(dv))))
-    dkv_walk<D, MODE, true>(a, ln, lds, stats, kf, vf, b, hk, wave, kb, kw, key, document, place, dk, dv);
-  if (key >= a.Nk) return;
-  if (!valid) {                                          // beyond the length: zeros
+    dkv_walk<D, MODE, true>(a, ln, lds, stats, marks[wave], kf, vf, b, hk, wave, kb, kw, rt, key, document, place, dk, dv);
+  __syncthreads();
+  // The wavefront of the tiles' second halves hands its sums to that of the first.
+  float *join = reinterpret_cast<float *>(memory) + (wave & 1) * (JOIN / 2) + (threadIdx.x & 63);
+  if (rt) {
 #pragma unroll
-    for (int t = 0; t < D::DT; ++t) {
-      dk[t] = zeros16();
-      dv[t] = zeros16();
-    }
+    for (int t = 0; t < D::DT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        join[(t * 16 + r) * 64] = dk[t][r];
+        join[((D::DT + t) * 16 + r) * 64] = dv[t][r];
+      }
   }
+  __syncthreads();
+  if (rt || key >= a.Nk) return;
+#pragma unroll
+  for (int t = 0; t < D::DT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {                       // beyond the length: zeros
+      dk[t][r] = valid ? dk[t][r] + join[(t * 16 + r) * 64] : 0.f;
+      dv[t][r] = valid ? dv[t][r] + join[((D::DT + t) * 16 + r) * 64] : 0.f;
+    }
   store_column<D>(static_cast<bf16 *>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2], a.D, dk, a.scale, ln.half);
   store_column<D>(static_cast<bf16 *>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2], a.Dv, dv, 1.f, ln.half);
 }
@@ -637,7 +675,7 @@ int sequence_splits(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk) {
   const int64_t columns = H / Hk * Nq;
   const int64_t items = columns <= 32 ? B * Hk : B * Hk * ceil_div(columns, int64_t(kColumns));
   const int64_t most = columns <= 32 ? ceil_div(Nk, int64_t(256)) : ceil_div(Nk, int64_t(512));
-  return int(std::max(int64_t(1), std::min(std::min(most, ceil_div(int64_t(512), items)), int64_t(64))));
+  return int(std::max(int64_t(1), std::min(std::min(most, 512 / items), int64_t(64))));
 }
 
 int64_t sequence_parts_bytes(int64_t B, int64_t H, int64_t Nq, int64_t Dv, int splits) {
@@ -658,12 +696,12 @@ int sequence_bf16_forward(const SequenceArgs &a, void *parts_memory, int splits,
     return check_launch("sequence_attention");
   }));
   if (splits <= 1) return XFH_OK;
-  join_kernel<<<dim3(unsigned(ceil_div(int64_t(a.B) * a.H * a.Nq * a.Dv, int64_t(256)))), 256, 0, s>>>(a, parts);
+  join_kernel<<<dim3(unsigned(ceil_div(int64_t(a.B) * a.H * a.Nq * (a.Dv / 4), int64_t(256)))), 256, 0, s>>>(a, parts);
   return check_launch("sequence_attention");
 }
 
 int sequence_bf16_backward(const SequenceArgs &a, hipStream_t s) {
-  const int64_t blocks = ceil_div(int64_t(a.H / a.Hk) * a.Nq, int64_t(kColumns)), kblocks = ceil_div(int64_t(a.Nk), int64_t(kColumns));
+  const int64_t blocks = ceil_div(int64_t(a.H / a.Hk) * a.Nq, int64_t(kColumns)), kblocks = ceil_div(int64_t(a.Nk), int64_t(kKeys));
   return with_dims(a, [&](auto dim, auto mode) {
     typedef decltype(dim) D;
     constexpr int MODE = decltype(mode)::value;
