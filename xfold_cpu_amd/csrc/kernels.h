@@ -317,7 +317,7 @@ struct SequenceArgs {
 };
 int64_t sequence_ranges_bytes(int64_t B, int64_t Nk);
 int sequence_ranges(const SequenceArgs &a, hipStream_t s);
-// bf16 (sequence_bf16.hip): the keys of a forward pass with few workgroups are split, their parts joined.
+// bf16 (sequence_bf16_forward.hip, sequence_bf16_backward.hip): the keys of a forward pass with few workgroups are split, their parts joined.
 int sequence_splits(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk);
 int64_t sequence_parts_bytes(int64_t B, int64_t H, int64_t Nq, int64_t Dv, int splits);
 bool sequence_bf16_forward_fits(const SequenceArgs &a);

@@ -1,4 +1,4 @@
-// Sequence attention for any head dim up to 128, in fp32 and for the bf16 layouts that sequence_bf16.hip does
+// Sequence attention for any head dim up to 128, in fp32 and for the bf16 layouts that sequence_bf16_forward.hip and sequence_bf16_backward.hip do
 // not take (rows that are not whole 16-byte pieces): forward, dq, dk and dv.
 //
 // A workgroup owns 64 tokens (16 per wavefront, one per lane column): queries in the forward pass and

@@ -7,11 +7,14 @@
 //
 // A tile of 64 tokens lies row-major in LDS, DL elements a row, brought there by direct loads (a
 // wavefront writes 1 KB, lane i its bytes [16 i, 16 i + 16)). 16-byte chunk c of row r is at slot
-// c ^ 2 ((r / RPB) % PAIRS): the 8 rows that one cycle of a row-fragment read takes, and the 8 rows that
-// the transposing reads of a wavefront take, are then in different banks. What lies beyond a
+// c ^ swizzle(r), chosen so that the 16 rows (one chunk each) of a row-fragment read, and the 4 rows (4
+// chunks each) of a transposing read, lie in different banks (256 bytes). What lies beyond a
 // matrix's end is a copy of its last row, beyond the head dim a copy of the row's first chunk: both
 // meet weights, or elements of the other operand, that are zero.
 #pragma once
+
+#include <algorithm>
+#include <type_traits>
 
 #include "sequence.h"
 
@@ -27,12 +30,13 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 // Head dims up to DL_ in LDS, KS_ steps of 16 in a product over the head dim, DT_ tiles of 32 of it in a result.
 template <int DL_, int KS_, int DT_> struct Dim {
   static constexpr int DL = DL_, KS = KS_, DT = DT_;
-  static constexpr int RPB = 128 / DL, PAIRS = DL / 16;
   static constexpr int ROW_PIECES = 512 / DL;            // rows of a 1 KB piece
   static constexpr int PIECES = kTile / ROW_PIECES;      // pieces of a tile of 64
   static_assert(DL == 32 || DL == 64 || DL == 128, "LDS rows of 64, 128 or 256 bytes");
   static_assert(KS * 16 <= DL && DT * 32 <= DL, "products within the row");
-  static __device__ __forceinline__ int swizzle(int row) { return 2 * ((row / RPB) & (PAIRS - 1)); }
+  static __device__ __forceinline__ int swizzle(int row) {
+    return (DL == 128 ? (row & 3) << 2 : DL == 64 ? (row & 2) << 1 : 0) | ((row >> 2) & 3);
+  }
 };
 
 __device__ __forceinline__ f32x16 mfma32(const bf16x8 &a, const bf16x8 &b, const f32x16 &c) {
@@ -49,45 +53,59 @@ __device__ __forceinline__ constexpr int row_of_register(int r) { return 8 * (r 
 
 // Lane offsets (elements) into a tile.
 template <class D> struct Lane {
-  int half, col, rows, swz, tr[D::DT];
+  int half, col, rows, swz, tr[2][D::DT];
   __device__ __forceinline__ Lane() {
     const int lane = threadIdx.x & 63;
     half = lane >> 5;
     col = lane & 31;
     rows = col * D::DL;
-    swz = D::swizzle(col);
-    // Transposing read: 16 lanes take 4 rows of 16 elements, 4 elements a lane.
-    const int i = lane & 15, row = 4 * half + i / 4, chunk = 2 * ((lane >> 4) & 1) + (i % 4) / 2;
+    swz = D::swizzle(col) ^ half;
+    // Transposing read: 16 lanes take 4 rows of 16 elements, 4 elements a lane; then the same 8 rows on.
+    const int i = lane & 15, chunk = 2 * ((lane >> 4) & 1) + (i % 4) / 2;
 #pragma unroll
-    for (int t = 0; t < D::DT; ++t) tr[t] = row * D::DL + ((t * 4 + chunk) ^ D::swizzle(row)) * 8 + 4 * (i & 1);
+    for (int s = 0; s < 2; ++s) {
+      const int row = 8 * s + 4 * half + i / 4;
+#pragma unroll
+      for (int t = 0; t < D::DT; ++t) tr[s][t] = row * D::DL + ((t * 4 + chunk) ^ D::swizzle(row)) * 8 + 4 * (i & 1);
+    }
   }
   // Rows 32 rt .. of a tile, elements 16 ks + 8 half ..: the A operand of a product over the head dim.
   __device__ __forceinline__ bf16x8 row_fragment(const bf16 *tile, int rt, int ks) const {
-    return *reinterpret_cast<const bf16x8 *>(tile + rt * 32 * D::DL + rows + (((2 * ks) ^ swz) + half) * 8);
+    return *reinterpret_cast<const bf16x8 *>(tile + rt * 32 * D::DL + rows + ((2 * ks) ^ swz) * 8);
   }
   // Head dims 32 t .. as rows, 16 rows of the tile from 16 kk on as k: the A operand of a product over tokens.
   __device__ __forceinline__ bf16x8 transposed(const bf16 *tile, int t, int kk) const {
-    const bf16 *p = tile + kk * 16 * D::DL + tr[t];
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 8 * D::DL));
+    const bf16 *p = tile + kk * 16 * D::DL;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + tr[0][t]));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + tr[1][t]));
     const __attribute__((ext_vector_type(8))) short v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(bf16x8, v);
   }
-  // [rows of the tile] x [owned columns] over the head dim.
+  // The fragments of a product are all read before its first MFMA (`reads_first`): read one by one, each
+  // MFMA waits for the LDS.
+  __device__ __forceinline__ void row_fragments(const bf16 *tile, int rt, bf16x8 (&f)[D::KS]) const {
+#pragma unroll
+    for (int ks = 0; ks < D::KS; ++ks) f[ks] = row_fragment(tile, rt, ks);
+  }
+  // [32 rows of the tile] x [owned columns] over the head dim.
   __device__ __forceinline__ f32x16 product(const bf16 *tile, int rt, const bf16x8 (&own)[D::KS]) const {
     f32x16 acc = zeros16();
 #pragma unroll
     for (int ks = 0; ks < D::KS; ++ks) acc = mfma32(row_fragment(tile, rt, ks), own[ks], acc);
     return acc;
   }
-  // acc += tile^T w over the 16 rows from 16 kk on. STRICT: elements that are not finite are left
-  // out and added to the columns that see them (`seen`, 1 or 0): with SIGNS as what they are, else as NaN.
+  __device__ __forceinline__ void transposed_fragments(const bf16 *tile, int kk, bf16x8 (&f)[D::DT]) const {
+#pragma unroll
+    for (int t = 0; t < D::DT; ++t) f[t] = transposed(tile, t, kk);
+  }
+  // acc += fragments^T w over 16 rows of a tile. STRICT: elements that are not finite are left out
+  // and added to the columns that see them (`seen`, 1 or 0): with SIGNS as what they are, else as NaN.
   template <bool STRICT, bool SIGNS>
-  __device__ __forceinline__ void accumulate(const bf16 *tile, int kk, const bf16x8 &w, const bf16x8 &seen,
+  __device__ __forceinline__ void accumulate(const bf16x8 (&f)[D::DT], const bf16x8 &w, const bf16x8 &seen,
                                              f32x16 (&acc)[D::DT]) const {
 #pragma unroll
     for (int t = 0; t < D::DT; ++t) {
-      bf16x8 a = transposed(tile, t, kk);
+      bf16x8 a = f[t];
       if constexpr (STRICT) {
         bf16x8 up, down;
 #pragma unroll
@@ -109,6 +127,7 @@ template <class D> struct Lane {
     }
   }
 };
+__device__ __forceinline__ void reads_first() { __builtin_amdgcn_sched_barrier(0); }
 
 // 8 registers of a result, rounded, as the B operand of a step of 16.
 __device__ __forceinline__ bf16x8 weights(const f32x16 &w, int first) {
@@ -289,6 +308,64 @@ __device__ __forceinline__ uint32_t hide_keys(const SequenceArgs &a, const Marks
     }
   }
   return seen;
+}
+
+constexpr int kColumns = 128;                            // columns of a workgroup (32 per wavefront)
+
+// Whether a result holds anything that is not finite.
+template <class D> __device__ __forceinline__ bool any_bad(const f32x16 (&o)[D::DT]) {
+  bool bad = false;
+#pragma unroll
+  for (int t = 0; t < D::DT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) bad |= !(fabsf(o[t][r]) < INFINITY);
+  return bad;
+}
+
+// A column's result: dims 32 t + 8 j + 4 half .. + 3, four at a time.
+template <class D>
+__device__ __forceinline__ void store_column(bf16 *out, int dim, const f32x16 (&o)[D::DT], float scale, int half) {
+#pragma unroll
+  for (int t = 0; t < D::DT; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = t * 32 + 8 * j + 4 * half;
+      if (d < dim) {
+        bf16x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = static_cast<bf16>(o[t][4 * j + e] * scale);
+        *reinterpret_cast<bf16x4 *>(out + d) = v;
+      }
+    }
+}
+
+// ------------------------------------------------------------------------------ launches
+
+inline int mode_of(const SequenceArgs &a) { return (a.cap > 0.f ? 1 : 0) | (a.slopes || (a.cap <= 0.f && a.scale <= 0.f) ? 2 : 0); }
+
+// f(Dim, MODE) for the call's head dims and scores.
+template <class D, class F> int with_mode(int mode, F f) {
+  switch (mode) {
+    case 0: return f(D(), std::integral_constant<int, 0>());
+    case 1: return f(D(), std::integral_constant<int, 1>());
+    case 2: return f(D(), std::integral_constant<int, 2>());
+    default: return f(D(), std::integral_constant<int, 3>());
+  }
+}
+template <class F> int with_dims(const SequenceArgs &a, F f) {
+  const int d = std::max(a.D, a.Dv), mode = mode_of(a);
+  if (d <= 32) return with_mode<Dim<32, 2, 1>>(mode, f);
+  if (d <= 48) return with_mode<Dim<64, 3, 2>>(mode, f);
+  if (d <= 64) return with_mode<Dim<64, 4, 2>>(mode, f);
+  if (d <= 96) return with_mode<Dim<128, 6, 3>>(mode, f);
+  return with_mode<Dim<128, 8, 4>>(mode, f);
+}
+
+inline bool rows_fit(const void *p, const int64_t *strides, int64_t dim, int64_t unit) {
+  if (reinterpret_cast<uintptr_t>(p) % (2 * unit) || dim % unit) return false;
+  for (int i = 0; i < 3; ++i)
+    if (strides[i] % unit || strides[i] < 0) return false;
+  return strides[2] < (int64_t(1) << 24);                // 64 rows of a tile within 32-bit offsets
 }
 
 }  // namespace seq
