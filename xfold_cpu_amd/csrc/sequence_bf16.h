@@ -194,7 +194,13 @@ template <class D, int W, int ROWS = kTile> struct Loader {
   }
 };
 
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Waits for this wavefront's loads (vmcnt 0; the other counters as they are). By the builtin, which the compiler
+// counts: after a wait written in assembly it would wait again, for the loads issued since too.
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  asm volatile("" ::: "memory");
+}
 
 // How a score comes from a dot product: MODE bit 0 = cap, bit 1 = the general form without a cap (distance
 // slopes, or a scale that is not positive). Scores are in log 2 units; with MODE 0 what is held is the
