@@ -980,6 +980,7 @@ static int64_t sequence_carve(Carver &cv, SequencePlan &p, const SequenceArgs &a
   if (p.splits > 1) p.parts = cv.take(sequence_parts_bytes(a.B, a.H, a.Nq, a.Dv, p.splits));
   if (a.documents) p.ranges = cv.take(sequence_ranges_bytes(a.B, a.Nk));
   if (backward) {
+    if (dtype == XFH_BF16) p.parts = cv.take(sequence_bf16_backward_parts(a.B, a.H, a.Hk, a.Nq, a.Nk, a.D, a.Dv));
     p.delta = static_cast<float *>(cv.take(int64_t(a.B) * a.H * a.Nq * 4));
     if (slopes) p.slope_part = static_cast<float *>(cv.take(sequence_slope_part(a.B, a.H, a.Nq) * 4));
   }
@@ -1031,7 +1032,7 @@ int xfh_sequence_attention_backward(const XfhSequenceAttention *args, void *work
   a.ranges = p.ranges;
   a.delta = p.delta;
   a.slope_part = p.slope_part;
-  return sequence_backward(a, args->dtype, args->dslopes, as_stream(stream));
+  return sequence_backward(a, args->dtype, p.parts, args->dslopes, as_stream(stream));
 }
 
 }  // extern "C"

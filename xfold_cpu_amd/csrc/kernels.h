@@ -323,9 +323,10 @@ int64_t sequence_parts_bytes(int64_t B, int64_t H, int64_t Nq, int64_t Dv, int s
 bool sequence_bf16_forward_fits(const SequenceArgs &a);
 bool sequence_bf16_backward_fits(const SequenceArgs &a);
 int sequence_bf16_forward(const SequenceArgs &a, void *parts, int splits, hipStream_t s);
-int sequence_bf16_backward(const SequenceArgs &a, hipStream_t s);
+int64_t sequence_bf16_backward_parts(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk, int64_t D, int64_t Dv);
+int sequence_bf16_backward(const SequenceArgs &a, void *parts, hipStream_t s);
 int sequence_forward(const SequenceArgs &a, int dtype, void *parts, int splits, hipStream_t s);
 int64_t sequence_slope_part(int64_t B, int64_t H, int64_t Nq);   // floats
-int sequence_backward(const SequenceArgs &a, int dtype, float *dslopes, hipStream_t s);
+int sequence_backward(const SequenceArgs &a, int dtype, void *parts, float *dslopes, hipStream_t s);
 
 }  // namespace xfh

@@ -575,14 +575,14 @@ int sequence_forward(const SequenceArgs &a, int dtype, void *parts, int splits, 
 
 int64_t sequence_slope_part(int64_t B, int64_t H, int64_t Nq) { return H * B * Nq; }
 
-int sequence_backward(const SequenceArgs &a, int dtype, float *dslopes, hipStream_t s) {
+int sequence_backward(const SequenceArgs &a, int dtype, void *parts, float *dslopes, hipStream_t s) {
   if (a.B > 0 && a.Hk > 0) {
     XFH_TRY(check_grid(a));
     XFH_TRY(sequence_ranges(a, s));
     const int d = std::max(a.D, a.Dv);
     int status = XFH_OK;
 #define XFH_SEQ_BACKWARD(DP) status = dtype == XFH_BF16 ? launch_backward<bf16, DP>(a, s) : launch_backward<float, DP>(a, s)
-    if (dtype == XFH_BF16 && sequence_bf16_backward_fits(a)) status = sequence_bf16_backward(a, s);
+    if (dtype == XFH_BF16 && sequence_bf16_backward_fits(a)) status = sequence_bf16_backward(a, parts, s);
     else if (d <= 32) XFH_SEQ_BACKWARD(32);
     else if (d <= 64) XFH_SEQ_BACKWARD(64);
     else if (d <= 96) XFH_SEQ_BACKWARD(96);

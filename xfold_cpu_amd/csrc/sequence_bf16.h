@@ -81,12 +81,6 @@ template <class D> struct Lane {
     const __attribute__((ext_vector_type(8))) short v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(bf16x8, v);
   }
-  // The fragments of a product are all read before its first MFMA (`reads_first`): read one by one, each
-  // MFMA waits for the LDS.
-  __device__ __forceinline__ void row_fragments(const bf16 *tile, int rt, bf16x8 (&f)[D::KS]) const {
-#pragma unroll
-    for (int ks = 0; ks < D::KS; ++ks) f[ks] = row_fragment(tile, rt, ks);
-  }
   // [32 rows of the tile] x [owned columns] over the head dim.
   __device__ __forceinline__ f32x16 product(const bf16 *tile, int rt, const bf16x8 (&own)[D::KS]) const {
     f32x16 acc = zeros16();
@@ -98,36 +92,35 @@ template <class D> struct Lane {
 #pragma unroll
     for (int t = 0; t < D::DT; ++t) f[t] = transposed(tile, t, kk);
   }
-  // acc += fragments^T w over 16 rows of a tile. STRICT: elements that are not finite are left out
-  // and added to the columns that see them (`seen`, 1 or 0): with SIGNS as what they are, else as NaN.
-  template <bool STRICT, bool SIGNS>
-  __device__ __forceinline__ void accumulate(const bf16x8 (&f)[D::DT], const bf16x8 &w, const bf16x8 &seen,
-                                             f32x16 (&acc)[D::DT]) const {
-#pragma unroll
-    for (int t = 0; t < D::DT; ++t) {
-      bf16x8 a = f[t];
-      if constexpr (STRICT) {
-        bf16x8 up, down;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = static_cast<float>(a[e]);
-          const bool bad = !(fabsf(x) < INFINITY);
-          up[e] = bf16(bad && !(SIGNS && x < 0.f) ? 1.f : 0.f);
-          down[e] = bf16(bad && !(SIGNS && x > 0.f) ? 1.f : 0.f);
-          if (bad) a[e] = bf16(0.f);
-        }
-        const f32x16 ups = mfma32(up, seen, zeros16()), downs = mfma32(down, seen, zeros16());
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          if (ups[r] > 0.f) acc[t][r] += INFINITY;
-          if (downs[r] > 0.f) acc[t][r] -= INFINITY;
-        }
-      }
-      acc[t] = mfma32(a, w, acc[t]);
-    }
-  }
 };
-__device__ __forceinline__ void reads_first() { __builtin_amdgcn_sched_barrier(0); }
+// acc += fragments^T w over 16 rows of a tile. STRICT: elements that are not finite are left out and added to
+// the columns that see them (`seen`, 1 or 0): with SIGNS as what they are, else as NaN.
+template <bool STRICT, bool SIGNS, int T>
+__device__ __forceinline__ void add_product(const bf16x8 (&f)[T], const bf16x8 &w, const bf16x8 &seen, f32x16 (&acc)[T]) {
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    bf16x8 a = f[t];
+    if constexpr (STRICT) {
+      bf16x8 up, down;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = static_cast<float>(a[e]);
+        const bool bad = !(fabsf(x) < INFINITY);
+        up[e] = bf16(bad && !(SIGNS && x < 0.f) ? 1.f : 0.f);
+        down[e] = bf16(bad && !(SIGNS && x > 0.f) ? 1.f : 0.f);
+        if (bad) a[e] = bf16(0.f);
+      }
+      const f32x16 ups = mfma32(up, seen, zeros16()), downs = mfma32(down, seen, zeros16());
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if (ups[r] > 0.f) acc[t][r] += INFINITY;
+        if (downs[r] > 0.f) acc[t][r] -= INFINITY;
+      }
+    }
+    acc[t] = mfma32(a, w, acc[t]);
+  }
+}
+
 
 // 8 registers of a result, rounded, as the B operand of a step of 16.
 __device__ __forceinline__ bf16x8 weights(const f32x16 &w, int first) {
@@ -177,20 +170,16 @@ template <class D, int W, int ROWS = kTile> struct Loader {
     const int c = int(threadIdx.x & 63) % (D::DL / 8) ^ D::swizzle(row(j));
     return c * 8 < dim ? c : 0;
   }
-  // Rows from `first` (at most the last one) on.
+  // Piece j of the rows from `first` (at most the last one) on.
+  __device__ __forceinline__ void load_piece(bf16 *tile, int first, int j) const {
+    const char *p = reinterpret_cast<const char *>(base + int64_t(first) * stride) + offset[j];
+    if (first + ROWS - 1 > last)
+      p = reinterpret_cast<const char *>(base + int64_t(min(first + row(j), last)) * stride) + chunk(j) * 16;
+    __builtin_amdgcn_global_load_lds((global_void *)p, (lds_void *)(tile + (wave + j * W) * 512), 16, 0, 0);
+  }
   __device__ __forceinline__ void load(bf16 *tile, int first) const {
-    if (first + ROWS - 1 <= last) {
-      const char *p = reinterpret_cast<const char *>(base + int64_t(first) * stride);
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        __builtin_amdgcn_global_load_lds((global_void *)(p + offset[j]), (lds_void *)(tile + (wave + j * W) * 512), 16, 0, 0);
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const char *p = reinterpret_cast<const char *>(base + int64_t(min(first + row(j), last)) * stride) + chunk(j) * 16;
-        __builtin_amdgcn_global_load_lds((global_void *)p, (lds_void *)(tile + (wave + j * W) * 512), 16, 0, 0);
-      }
-    }
+    for (int j = 0; j < N; ++j) load_piece(tile, first, j);
   }
 };
 
@@ -319,20 +308,20 @@ __device__ __forceinline__ uint32_t hide_keys(const SequenceArgs &a, const Marks
 constexpr int kColumns = 128;                            // columns of a workgroup (32 per wavefront)
 
 // Whether a result holds anything that is not finite.
-template <class D> __device__ __forceinline__ bool any_bad(const f32x16 (&o)[D::DT]) {
+template <int T> __device__ __forceinline__ bool any_bad(const f32x16 (&o)[T]) {
   bool bad = false;
 #pragma unroll
-  for (int t = 0; t < D::DT; ++t)
+  for (int t = 0; t < T; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) bad |= !(fabsf(o[t][r]) < INFINITY);
   return bad;
 }
 
 // A column's result: dims 32 t + 8 j + 4 half .. + 3, four at a time.
-template <class D>
-__device__ __forceinline__ void store_column(bf16 *out, int dim, const f32x16 (&o)[D::DT], float scale, int half) {
+template <int T>
+__device__ __forceinline__ void store_column(bf16 *out, int dim, const f32x16 (&o)[T], float scale, int half) {
 #pragma unroll
-  for (int t = 0; t < D::DT; ++t)
+  for (int t = 0; t < T; ++t)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int d = t * 32 + 8 * j + 4 * half;

@@ -1,8 +1,7 @@
 // Sequence attention in bf16 on 32x32x16 MFMAs (sequence_bf16.h), backward: dq, then dk and dv.
 //
-// dq: the columns are queries, as in the forward pass. dk and dv: the columns are 64 keys, each 32 of them
-// with two wavefronts that take half a tile of queries each; the loop goes over the heads of the group
-// and their queries. Two kernels with 3 and 4 products, of which 2 are the same, in place of one with
+// dq: the columns are queries, as in the forward pass. dk and dv: the columns are 64 keys, the loop goes
+// over the heads of the group and their queries. Two kernels with 3 and 4 products, of which 2 are the same, in place of one with
 // 5: the sums of dq need no atomics, and a call gives the same bits every time.
 #include "sequence_bf16.h"
 
@@ -69,7 +68,7 @@ __device__ __forceinline__ void dq_walk(const SequenceArgs &a, const Lane<D> &ln
       for (int s = 0; s < 2; ++s) {
         bf16x8 tf[D::DT];
         ln.transposed_fragments(kt, 2 * rt + s, tf);
-        ln.template accumulate<STRICT, false>(tf, weights(w, 8 * s), weights_seen(seen, 8 * s), dq);
+        add_product<STRICT, false>(tf, weights(w, 8 * s), weights_seen(seen, 8 * s), dq);
       }
     }
   };
@@ -141,10 +140,10 @@ __global__ __launch_bounds__(256, 2) void dq_bf16_kernel(SequenceArgs a, int blo
   f32x16 dq[D::DT];
   SlopeSums sums;
   dq_walk<D, MODE, false>(a, ln, stage0, stage1, kl, vl, qf, gf, score, b, end, place.n, block, mine, row, marks[wave], lse, delta, dq, sums);
-  if (__syncthreads_or(valid && any_bad<D>(dq)))
+  if (__syncthreads_or(valid && any_bad(dq)))
     dq_walk<D, MODE, true>(a, ln, stage0, stage1, kl, vl, qf, gf, score, b, end, place.n, block, mine, row, marks[wave], lse, delta, dq, sums);
   if (valid)
-    store_column<D>(static_cast<bf16 *>(a.dq) + b * a.dqs[0] + h * a.dqs[1] + i * a.dqs[2], a.D, dq, a.scale, ln.half);
+    store_column(static_cast<bf16 *>(a.dq) + b * a.dqs[0] + h * a.dqs[1] + i * a.dqs[2], a.D, dq, a.scale, ln.half);
   if constexpr (Score<MODE>::SLOPE) {
     if (!a.slope_part) return;
     sums.far += other_half(sums.far);
@@ -184,25 +183,40 @@ __device__ __forceinline__ uint32_t hide_queries(const Marks &marks, int half, i
   return seen;
 }
 
-constexpr int kKeys = 64;                                // keys of a workgroup: 2 groups of 32, each with 2 wavefronts
+constexpr int kKeys = 64;                                // keys of a workgroup
 
-// One wavefront: 32 keys from kw on, and of each tile of 64 queries the 32 from 32 rt on.
+// Tiles of LDS in use: with two, the next one is on its way during a step. At DL = 128 two would leave room for
+// one workgroup per CU; two workgroups with one stage each hide each other's loads.
+template <class D> constexpr int kDkvStages = D::DL == 128 ? 1 : 2;
+// The heads and tiles of queries of a work item, [head0, head1) and [tile0, tile1).
+struct Share { int head0, head1, tile0, tile1; };
+struct Splits { int heads, tiles; };
+
+// What the two wavefronts of a key group hand each other: P and dS of 32 queries as B fragments, and, in
+// the rare form, the bits of the pairs that are seen.
+struct Exchange { bf16x8 p[2][64], ds[2][64]; uint32_t seen[64]; };
+
+// Wavefront (key group kg, part): keys kw .. + 31. Of a tile of 64 queries it works out P and dS of the 32
+// from 32 part on, and it owns dims 16 DT part .. of dk and dv (half of them: the sums of a whole
+// head dim of 128 take 128 registers, and with the keys' own 64 leave room for one wavefront per SIMD
+// only). So it adds its own 32 queries' products, then, behind a barrier, its partner's.
 template <class D, int MODE, bool STRICT>
-__device__ __forceinline__ void dkv_walk(const SequenceArgs &a, const Lane<D> &ln, bf16 *stage0, bf16 *stage1,
-                                         float *stats0, float *stats1, Marks &marks, const bf16x8 (&kf)[D::KS],
-                                         const bf16x8 (&vf)[D::KS], int b, int hk, int wave, int kb, int kw, int rt, int key,
-                                         int document, const Place &place, f32x16 (&dk)[D::DT], f32x16 (&dv)[D::DT]) {
-  constexpr int TILE = kTile * D::DL;
-  const int group = a.H / a.Hk, qtiles = (a.Nq + kTile - 1) / kTile;
+__device__ __forceinline__ void dkv_walk(const SequenceArgs &a, const Lane<D> &ln, bf16 *stage0, bf16 *stage1, float *stats0,
+                                         float *stats1, Exchange *exchange, Marks &marks, const bf16x8 (&kf)[D::KS],
+                                         const bf16x8 (&vf)[D::KS], int b, int hk, int wave, int kb, int kw, int part, int key,
+                                         int document, const Place &place, const Share &share, f32x16 (&dk)[D::DT / 2],
+                                         f32x16 (&dv)[D::DT / 2]) {
+  constexpr int TILE = kTile * D::DL, T = D::DT / 2;
+  const int group = a.H / a.Hk, lane = threadIdx.x & 63;
 #pragma unroll
-  for (int t = 0; t < D::DT; ++t) {
+  for (int t = 0; t < T; ++t) {
     dk[t] = zeros16();
     dv[t] = zeros16();
   }
   Range range{0x7fffffff, -1, 0, 0};
   if (a.documents) range = static_cast<const Range *>(a.ranges)[int64_t(b) * a.tiles + kb / kTile];
   const auto test = [&](int tile) {
-    const int i0 = tile * kTile + rt * 32, i1 = min(i0 + 32, a.Nq) - 1, last = min(tile * kTile + kTile, a.Nq) - 1;
+    const int i0 = tile * kTile + part * 32, i1 = min(i0 + 32, a.Nq) - 1, last = min(tile * kTile + kTile, a.Nq) - 1;
     Needs n{limit_of(a, place, last) > kb, i0 <= i1 && limit_of(a, place, max(i1, 0)) > kw,
             i0 + 32 <= a.Nq && limit_of(a, place, i0) >= kw + 32};
     if (a.documents && n.block) {
@@ -212,81 +226,97 @@ __device__ __forceinline__ void dkv_walk(const SequenceArgs &a, const Lane<D> &l
     }
     return n;
   };
-  for (int g = 0; g < group; ++g) {
+  for (int g = share.head0; g < share.head1; ++g) {
     const int h = hk * group + g;
     const Score<MODE> score(a, h);
     const Loader<D, 4> ql(static_cast<const bf16 *>(a.q) + b * a.qs[0] + h * a.qs[1], a.qs[2], a.Nq, a.D, wave);
     const Loader<D, 4> gl(static_cast<const bf16 *>(a.dout) + b * a.gs[0] + h * a.gs[1], a.gs[2], a.Nq, a.Dv, wave);
     const int64_t at = (int64_t(b) * a.H + h) * a.Nq;
-    const auto load = [&](bf16 *to, float *stats, int tile) {
-      ql.load(to, tile * kTile);
-      gl.load(to + TILE, tile * kTile);
+    Walk walk(share.tile0, share.tile1);
+    Step now = walk.next(test);
+    const auto load = [&](bf16 *stage, float *stats, int tile) {
+      ql.load(stage, tile * kTile);
+      gl.load(stage + TILE, tile * kTile);
       if (wave < 2) {                                    // 64 lse, 64 delta (beyond the end: the last one's)
-        const float *from = (wave ? a.delta : a.lse) + at + min(tile * kTile + int(threadIdx.x & 63), a.Nq - 1);
+        const float *from = (wave ? a.delta : a.lse) + at + min(tile * kTile + lane, a.Nq - 1);
         __builtin_amdgcn_global_load_lds((global_void *)from, (lds_void *)(stats + wave * kTile), 4, 0, 0);
       }
     };
-    Walk walk(0, qtiles);
-    Step now = walk.next(test);
     const auto compute = [&](const bf16 *qt, const float *stats) {
-      if (!now.mine) return;
       const bf16 *gt = qt + TILE;
-      const float *lses = stats + rt * 32, *deltas = lses + kTile;
-      const int i0 = now.tile * kTile + rt * 32;
-      if (!now.whole) mark_queries(a, place, b, i0, marks);
-      f32x16 w = zeros16(), dp = zeros16(), bent;
-      bf16x8 qf[D::KS], gf[D::KS], qtf[2][D::DT], gtf[2][D::DT];
-      ln.row_fragments(qt, rt, qf);
-      ln.row_fragments(gt, rt, gf);
-      reads_first();
+      // acc += transposed rows (steps of 16 from 2 half on) times the fragments of P and dS.
+      const auto add = [&](int half, const bf16x8 (&p)[2], const bf16x8 (&ds)[2], uint32_t seen) {
 #pragma unroll
-      for (int ks = 0; ks < D::KS; ++ks) {
-        w = mfma32(qf[ks], kf[ks], w);
-        dp = mfma32(gf[ks], vf[ks], dp);
-      }
-      ln.transposed_fragments(gt, 2 * rt, gtf[0]);
-      ln.transposed_fragments(qt, 2 * rt, qtf[0]);
-      const float gap = float(i0 + place.shift + 4 * ln.half - key);
+        for (int s = 0; s < 2; ++s) {
+          const bf16x8 sf = weights_seen(seen, 8 * s);
+          bf16x8 f[T];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float f = 1.f;
-        w[r] = score(w[r], gap + float(row_of_register(r)), &f);
-        if constexpr (Score<MODE>::CAP) bent[r] = f;
-      }
-      uint32_t seen = 0xffff;
-      if (!now.whole) seen = hide_queries(marks, ln.half, key, document, w);
-      ln.transposed_fragments(gt, 2 * rt + 1, gtf[1]);
-      ln.transposed_fragments(qt, 2 * rt + 1, qtf[1]);
+          for (int t = 0; t < T; ++t) f[t] = ln.transposed(gt, part * T + t, 2 * half + s);
+          add_product<STRICT, false>(f, p[s], sf, dv);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 lse = *reinterpret_cast<const f32x4 *>(lses + 8 * j + 4 * ln.half);
-        const f32x4 delta = *reinterpret_cast<const f32x4 *>(deltas + 8 * j + 4 * ln.half);
+          for (int t = 0; t < T; ++t) f[t] = ln.transposed(qt, part * T + t, 2 * half + s);
+          add_product<STRICT, false>(f, ds[s], sf, dk);
+        }
+      };
+      uint32_t seen = 0;
+      bf16x8 pf[2] = {}, dsf[2] = {};
+      if (now.mine) {
+        if (!now.whole) mark_queries(a, place, b, now.tile * kTile + part * 32, marks);
+        const float *lses = stats + part * 32, *deltas = lses + kTile;
+        f32x16 w = ln.product(qt, part, kf), dp = ln.product(gt, part, vf), bent;
+        const float gap = float(now.tile * kTile + part * 32 + place.shift + 4 * ln.half - key);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * j + e;
-          const bool see = now.whole || ((seen >> r) & 1);
-          const float p = see ? score.weight(w[r], lse[e]) : 0.f;
-          float ds = see ? p * (dp[r] - delta[e]) : 0.f;
-          if constexpr (Score<MODE>::CAP) ds *= bent[r];
-          w[r] = p;
-          dp[r] = ds;
+        for (int r = 0; r < 16; ++r) {
+          float f = 1.f;
+          w[r] = score(w[r], gap + float(row_of_register(r)), &f);
+          if constexpr (Score<MODE>::CAP) bent[r] = f;
+        }
+        seen = now.whole ? 0xffff : hide_queries(marks, ln.half, key, document, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 lse = *reinterpret_cast<const f32x4 *>(lses + 8 * j + 4 * ln.half);
+          const f32x4 delta = *reinterpret_cast<const f32x4 *>(deltas + 8 * j + 4 * ln.half);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * j + e;
+            const bool see = now.whole || ((seen >> r) & 1);
+            const float p = see ? score.weight(w[r], lse[e]) : 0.f;
+            float ds = see ? p * (dp[r] - delta[e]) : 0.f;
+            if constexpr (Score<MODE>::CAP) ds *= bent[r];
+            w[r] = p;
+            dp[r] = ds;
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          pf[s] = weights(w, 8 * s);
+          dsf[s] = weights(dp, 8 * s);
         }
       }
+      Exchange &mine = exchange[wave];
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const bf16x8 sf = weights_seen(seen, 8 * s);
-        ln.template accumulate<STRICT, false>(gtf[s], weights(w, 8 * s), sf, dv);
-        ln.template accumulate<STRICT, false>(qtf[s], weights(dp, 8 * s), sf, dk);
+        mine.p[s][lane] = pf[s];
+        mine.ds[s][lane] = dsf[s];
       }
+      if constexpr (STRICT) mine.seen[lane] = seen;
+      add(part, pf, dsf, seen);
+      ring_barrier();
+      const Exchange &other = exchange[wave ^ 2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        pf[s] = other.p[s][lane];
+        dsf[s] = other.ds[s][lane];
+      }
+      add(part ^ 1, pf, dsf, STRICT ? other.seen[lane] : 0);
     };
-    if constexpr (STRICT) {                              // rare: one stage will do
-      while (now.tile >= 0) {
-        ring_barrier();
+    if constexpr (STRICT || kDkvStages<D> == 1) {
+      for (; now.tile >= 0; now = walk.next(test)) {
+        ring_barrier();                                  // the tile before is no longer read
         load(stage0, stats0, now.tile);
         wait_loads();
         ring_barrier();
         compute(stage0, stats0);
-        now = walk.next(test);
       }
     } else {
       const auto step = [&](bf16 *use, float *use_stats, bf16 *spare, float *spare_stats) {
@@ -308,15 +338,25 @@ __device__ __forceinline__ void dkv_walk(const SequenceArgs &a, const Lane<D> &l
   }
 }
 
+// Work item = (split, key block, batch entry, key head); the sums of split s go to parts [s][B Hk][Nk][D + Dv] in
+// fp32 when there are several.
 template <class D, int MODE>
-__global__ __launch_bounds__(256, D::DL == 128 ? 1 : 2) void dkv_bf16_kernel(SequenceArgs a, int blocks) {
-  constexpr int TILE = kTile * D::DL;
-  __shared__ __attribute__((aligned(1024))) bf16 stage0[2 * TILE], stage1[2 * TILE];
-  __shared__ __attribute__((aligned(1024))) float stats0[2 * kTile], stats1[2 * kTile];
+__global__ __launch_bounds__(256, 2) void dkv_bf16_kernel(SequenceArgs a, Splits splits, float *parts) {
+  constexpr int TILE = kTile * D::DL, T = D::DT / 2, STAGES = kDkvStages<D>;
+  static_assert(D::DT % 2 == 0, "two wavefronts share the head dim");
+  __shared__ __attribute__((aligned(1024))) bf16 stage0[2 * TILE], stage1[STAGES == 2 ? 2 * TILE : 8];
+  __shared__ __attribute__((aligned(1024))) float stats0[2 * kTile], stats1[STAGES == 2 ? 2 * kTile : 4];
+  __shared__ __attribute__((aligned(16))) Exchange exchange[4];
   __shared__ __attribute__((aligned(16))) Marks marks[4];
-  static_assert(sizeof(stage0) >= 2 * D::DT * 16 * 64 * 4, "a key group's sums are joined in a stage");
-  const int hk = blockIdx.x % a.Hk, rest = blockIdx.x / a.Hk, blk = rest % blocks, b = rest / blocks;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rt = wave >> 1;
+  const int hk = blockIdx.x % a.Hk;
+  int rest = blockIdx.x / a.Hk;
+  const int b = rest % a.B;
+  rest /= a.B;
+  const int count = splits.heads * splits.tiles, split = rest % count, blk = rest / count;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave >> 1;
+  const int group = a.H / a.Hk, qtiles = (a.Nq + kTile - 1) / kTile, sh = split % splits.heads, st = split / splits.heads;
+  const Share share{sh * group / splits.heads, (sh + 1) * group / splits.heads, int(int64_t(st) * qtiles / splits.tiles),
+                    int(int64_t(st + 1) * qtiles / splits.tiles)};
   const Lane<D> ln;
   const Place place = place_of(a, b);
   const int kb = blk * kKeys, kw = kb + (wave & 1) * 32, key = kw + ln.col;
@@ -326,33 +366,65 @@ __global__ __launch_bounds__(256, D::DL == 128 ? 1 : 2) void dkv_bf16_kernel(Seq
   own_row<D>(vf, static_cast<const bf16 *>(a.v) + b * a.vs[0] + hk * a.vs[1] + key * a.vs[2], a.Dv, valid, ln.half);
   int document = 0;                                      // (as row_of has it without documents)
   if (a.documents) document = valid ? a.documents[int64_t(b) * a.documents_stride + key] : -1;
-  f32x16 dk[D::DT], dv[D::DT];
-  dkv_walk<D, MODE, false>(a, ln, stage0, stage1, stats0, stats1, marks[wave], kf, vf, b, hk, wave, kb, kw, rt, key, document, place, dk, dv);
-  if (__syncthreads_or(valid && (any_bad<D>(dk) || any_bad<D>(dv))))
-    dkv_walk<D, MODE, true>(a, ln, stage0, stage1, stats0, stats1, marks[wave], kf, vf, b, hk, wave, kb, kw, rt, key, document, place, dk, dv);
-  __syncthreads();
-  // The wavefront of the tiles' second halves hands its sums to that of the first.
-  float *join = reinterpret_cast<float *>(wave & 1 ? stage1 : stage0) + (threadIdx.x & 63);
-  if (rt) {
+  f32x16 dk[T], dv[T];
+  dkv_walk<D, MODE, false>(a, ln, stage0, stage1, stats0, stats1, exchange, marks[wave], kf, vf, b, hk, wave, kb, kw, part, key,
+                           document, place, share, dk, dv);
+  if (__syncthreads_or(valid && (any_bad(dk) || any_bad(dv))))
+    dkv_walk<D, MODE, true>(a, ln, stage0, stage1, stats0, stats1, exchange, marks[wave], kf, vf, b, hk, wave, kb, kw, part, key,
+                            document, place, share, dk, dv);
+  if (key >= a.Nk) return;
+  if (!valid) {                                          // beyond the length: zeros
 #pragma unroll
-    for (int t = 0; t < D::DT; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        join[(t * 16 + r) * 64] = dk[t][r];
-        join[((D::DT + t) * 16 + r) * 64] = dv[t][r];
-      }
-  }
-  __syncthreads();
-  if (rt || key >= a.Nk) return;
-#pragma unroll
-  for (int t = 0; t < D::DT; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {                       // beyond the length: zeros
-      dk[t][r] = valid ? dk[t][r] + join[(t * 16 + r) * 64] : 0.f;
-      dv[t][r] = valid ? dv[t][r] + join[((D::DT + t) * 16 + r) * 64] : 0.f;
+    for (int t = 0; t < T; ++t) {
+      dk[t] = zeros16();
+      dv[t] = zeros16();
     }
-  store_column<D>(static_cast<bf16 *>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2], a.D, dk, a.scale, ln.half);
-  store_column<D>(static_cast<bf16 *>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2], a.Dv, dv, 1.f, ln.half);
+  }
+  const int d0 = part * T * 32;
+  if (count > 1) {
+    float *to = parts + ((int64_t(split) * a.B * a.Hk + int64_t(b) * a.Hk + hk) * a.Nk + key) * (a.D + a.Dv);
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = d0 + t * 32 + 8 * j + 4 * ln.half;
+        if (d < a.D) *reinterpret_cast<f32x4 *>(to + d) = f32x4{dk[t][4 * j], dk[t][4 * j + 1], dk[t][4 * j + 2], dk[t][4 * j + 3]};
+        if (d < a.Dv)
+          *reinterpret_cast<f32x4 *>(to + a.D + d) = f32x4{dv[t][4 * j], dv[t][4 * j + 1], dv[t][4 * j + 2], dv[t][4 * j + 3]};
+      }
+    return;
+  }
+  store_column(static_cast<bf16 *>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2] + d0, a.D - d0, dk, a.scale, ln.half);
+  store_column(static_cast<bf16 *>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2] + d0, a.Dv - d0, dv, 1.f, ln.half);
+}
+
+// dk and dv from the parts of their work items, in order: a thread per 4 elements.
+__global__ __launch_bounds__(256) void dkv_join_kernel(SequenceArgs a, int splits, const float *parts) {
+  const int width = a.D + a.Dv, quads = width / 4;
+  const int64_t rows = int64_t(a.B) * a.Hk * a.Nk, at = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= rows * quads) return;
+  const int64_t row = at / quads;
+  const int d = int(at - row * quads) * 4;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const f32x4 *>(parts + (s * rows + row) * width + d);
+  const int key = int(row % a.Nk), bk = int(row / a.Nk), hk = bk % a.Hk, b = bk / a.Hk;
+  bf16 *out = d < a.D ? static_cast<bf16 *>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2] + d
+                      : static_cast<bf16 *>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2] + d - a.D;
+  const float scale = d < a.D ? a.scale : 1.f;
+  bf16x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = static_cast<bf16>(sum[e] * scale);
+  *reinterpret_cast<bf16x4 *>(out) = v;
+}
+
+// Parts of the heads and of the queries that dk and dv are summed in: at least about 1024 work items (two rounds
+// of two workgroups per CU), so that long and short ones even out.
+Splits dkv_splits(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk) {
+  if (B == 0 || Hk == 0 || H == 0 || Nk == 0) return {1, 1};
+  const int64_t items = ceil_div(Nk, int64_t(kKeys)) * B * Hk, want = std::max(int64_t(1), 1024 / items);
+  const int64_t heads = std::min(H / Hk, want);
+  const int64_t tiles = std::max(int64_t(1), std::min(want / heads, ceil_div(Nq, int64_t(4 * kTile))));
+  return {int(heads), int(std::min(tiles, int64_t(16)))};
 }
 
 }  // namespace
@@ -363,14 +435,27 @@ bool sequence_bf16_backward_fits(const SequenceArgs &a) {
 }
 
 
-int sequence_bf16_backward(const SequenceArgs &a, hipStream_t s) {
+int64_t sequence_bf16_backward_parts(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk, int64_t D, int64_t Dv) {
+  const Splits n = dkv_splits(B, H, Hk, Nq, Nk);
+  return n.heads * n.tiles <= 1 ? 0 : int64_t(n.heads) * n.tiles * B * Hk * Nk * (D + Dv) * 4;
+}
+
+int sequence_bf16_backward(const SequenceArgs &a, void *parts, hipStream_t s) {
   const int64_t blocks = ceil_div(int64_t(a.H / a.Hk) * a.Nq, int64_t(kColumns)), kblocks = ceil_div(int64_t(a.Nk), int64_t(kKeys));
   return with_dims(a, [&](auto dim, auto mode) {
     typedef decltype(dim) D;
     constexpr int MODE = decltype(mode)::value;
     if (blocks > 0) dq_bf16_kernel<D, MODE><<<dim3(unsigned(blocks * a.Hk * a.B)), 256, 0, s>>>(a, int(blocks));
     XFH_TRY(check_launch("sequence_attention_backward"));
-    if (kblocks > 0) dkv_bf16_kernel<D, MODE><<<dim3(unsigned(kblocks * a.Hk * a.B)), 256, 0, s>>>(a, int(kblocks));
+    typedef Dim<D::DL < 64 ? 64 : D::DL, D::KS, D::DT + D::DT % 2> E;    // (two wavefronts share the head dim)
+    if (kblocks == 0) return int(XFH_OK);
+    const Splits splits = dkv_splits(a.B, a.H, a.Hk, a.Nq, a.Nk);
+    const int count = splits.heads * splits.tiles;
+    dkv_bf16_kernel<E, MODE><<<dim3(unsigned(kblocks * a.Hk * a.B * count)), 256, 0, s>>>(a, splits, static_cast<float *>(parts));
+    XFH_TRY(check_launch("sequence_attention_backward"));
+    if (count > 1)
+      dkv_join_kernel<<<dim3(unsigned(ceil_div(int64_t(a.B) * a.Hk * a.Nk * ((a.D + a.Dv) / 4), int64_t(256)))), 256, 0, s>>>(
+          a, count, static_cast<const float *>(parts));
     return check_launch("sequence_attention_backward");
   });
 }

@@ -61,7 +61,7 @@ __device__ __forceinline__ void forward_tile(const SequenceArgs &a, const Lane<D
   for (int kk = 0; kk < 2 * RT; ++kk) {
     bf16x8 vf[D::DT];
     ln.transposed_fragments(vt, kk, vf);
-    ln.template accumulate<STRICT, true>(vf, weights(w[kk / 2], 8 * (kk & 1)), weights_seen(seen[kk / 2], 8 * (kk & 1)), o);
+    add_product<STRICT, true>(vf, weights(w[kk / 2], 8 * (kk & 1)), weights_seen(seen[kk / 2], 8 * (kk & 1)), o);
   }
 }
 
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(256, 2) void forward_bf16_kernel(SequenceArgs a, in
   f32x16 o[D::DT];
   float m, l;
   forward_walk<D, MODE, false>(a, ln, stage0, stage1, kl, vl, qf, score, b, first, end, place.n, block, mine, row, marks[wave], m, l, o);
-  if (__syncthreads_or(valid && any_bad<D>(o)))
+  if (__syncthreads_or(valid && any_bad(o)))
     forward_walk<D, MODE, true>(a, ln, stage0, stage1, kl, vl, qf, score, b, first, end, place.n, block, mine, row, marks[wave], m, l, o);
   l += other_half(l);
   if (!valid) return;
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256, 2) void forward_bf16_kernel(SequenceArgs a, in
       }
     return;
   }
-  store_column<D>(static_cast<bf16 *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2], a.Dv, o, l == 0.f ? 0.f : 1.0f / l, ln.half);
+  store_column(static_cast<bf16 *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2], a.Dv, o, l == 0.f ? 0.f : 1.0f / l, ln.half);
   if (a.lse && ln.half == 0) a.lse[(int64_t(b) * a.H + h) * a.Nq + i] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, int 
   f32x16 o[D::DT];
   float m, l;
   token_walk<D, MODE, false>(a, ln, stage0[wave], stage1[wave], kl, vl, qf, score, b, first + wave, end, place.n, span, row, marks[wave], m, l, o);
-  if (__syncthreads_or(valid && any_bad<D>(o)))
+  if (__syncthreads_or(valid && any_bad(o)))
     token_walk<D, MODE, true>(a, ln, stage0[wave], stage1[wave], kl, vl, qf, score, b, first + wave, end, place.n, span, row, marks[wave], m, l, o);
   l += other_half(l);
   __syncthreads();
