@@ -26,17 +26,49 @@ def _rows(t: torch.Tensor, cols: int):
     return t, cols
 
 
+_CODES = {torch.float32: nh.F32, torch.bfloat16: nh.BF16}
+
+
+def _arg(t: Optional[torch.Tensor]):
+    """Address and type of a parameter vector for the library."""
+    return (None, nh.F32) if t is None else (t.data_ptr(), _CODES[t.dtype])
+
+
 def _forward(x, cols, weight, bias, eps, out_dtype, keep):
     x, stride = _rows(x, cols)
+    device = x.device
     rows = x.numel() // cols if cols else 0
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if keep else None
-    with nh.on_device(x.device):
-        nh.call("xfh_layer_norm_train", nh.ptr(x), nh.dtype_code(x.dtype), stride, rows, cols, nh.ptr(weight),
-                nh.F32 if weight is None else nh.dtype_code(weight.dtype), nh.ptr(bias),
-                nh.F32 if bias is None else nh.dtype_code(bias.dtype), eps, nh.ptr(y), nh.dtype_code(out_dtype),
-                nh.ptr(stats), nh.stream_of(x.device))
+    y = torch.empty(x.shape, dtype=out_dtype, device=device)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=device) if keep else None
+    nh.launch(device, "xfh_layer_norm_train", x.data_ptr(), _CODES[x.dtype], stride, rows, cols, *_arg(weight),
+              *_arg(bias), eps, y.data_ptr(), _CODES[out_dtype], None if stats is None else stats.data_ptr())
     return x, y, stats
+
+
+def _backward(ctx, dy):
+    x, weight, stats = ctx.saved_tensors
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    cols, out_dtype, bias = ctx.call
+    device = x.device
+    if dy.dtype != out_dtype:
+        dy = dy.to(out_dtype)
+    dy, dy_stride = _rows(dy, cols)
+    x, x_stride = _rows(x, cols)
+    rows = stats.shape[0]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
+    dw = torch.empty_like(weight) if need_w else None
+    db = torch.empty(bias[0], dtype=bias[1], device=device) if need_b else None
+    ws, size = None, 0
+    if need_w or need_b:
+        size = nh.function("xfh_layer_norm_backward_workspace_size")(rows, cols)
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+    nh.launch(device, "xfh_layer_norm_backward", dy.data_ptr(), _CODES[out_dtype], dy_stride, x.data_ptr(),
+              _CODES[x.dtype], x_stride, rows, cols, *_arg(weight), stats.data_ptr(),
+              None if dx is None else dx.data_ptr(), *_arg(dw), *_arg(db), None if ws is None else ws.data_ptr(), size)
+    return dx, dw, db, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _TrainableLayerNorm(torch.autograd.Function):
@@ -45,35 +77,13 @@ class _TrainableLayerNorm(torch.autograd.Function):
         w = None if weight is None else weight.contiguous()
         x, y, stats = _forward(x, cols, w, None if bias is None else bias.contiguous(), eps, out_dtype, True)
         ctx.save_for_backward(x, w, stats)
-        ctx.cols, ctx.out_dtype = cols, out_dtype
-        ctx.bias_of = None if bias is None else (bias.shape, bias.dtype)
+        ctx.call = cols, out_dtype, None if bias is None else (bias.shape, bias.dtype)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        cols, device = ctx.cols, x.device
-        if dy.dtype != ctx.out_dtype:
-            dy = dy.to(ctx.out_dtype)
-        dy, dy_stride = _rows(dy, cols)
-        x, x_stride = _rows(x, cols)
-        rows = x.numel() // cols if cols else 0
-        dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
-        dw = torch.empty_like(weight) if need_w else None
-        db = torch.empty(ctx.bias_of[0], dtype=ctx.bias_of[1], device=device) if need_b else None
-        with nh.on_device(device):
-            ws = None
-            if need_w or need_b:
-                ws = nh.workspace(nh.load_library().xfh_layer_norm_backward_workspace_size(rows, cols), device)
-            nh.call("xfh_layer_norm_backward", nh.ptr(dy), nh.dtype_code(dy.dtype), dy_stride, nh.ptr(x),
-                    nh.dtype_code(x.dtype), x_stride, rows, cols, nh.ptr(weight),
-                    nh.F32 if weight is None else nh.dtype_code(weight.dtype), nh.ptr(stats), nh.ptr(dx), nh.ptr(dw),
-                    nh.F32 if dw is None else nh.dtype_code(dw.dtype), nh.ptr(db),
-                    nh.F32 if db is None else nh.dtype_code(db.dtype), nh.ptr(ws), 0 if ws is None else ws.numel(),
-                    nh.stream_of(device))
-        return dx, dw, db, None, None, None
+        # Gradients that are to be differentiated again get the node that refuses it.
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
 def trainable_layer_norm(x: torch.Tensor, normalized_shape, weight: Optional[torch.Tensor] = None,

@@ -19,7 +19,6 @@ runs in the library's HIP kernels.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import os
@@ -105,6 +104,10 @@ SIGNATURES = {
 }
 
 
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 class HipBackendError(RuntimeError):
     """A libxfold_hip call returned an error status."""
 
@@ -162,6 +165,21 @@ def call(name: str, *args) -> None:
         raise HipBackendError(f"{name} failed ({status}): {message}")
 
 
+@functools.lru_cache(maxsize=None)
+def function(name: str):
+    return getattr(load_library(), name)
+
+
+def launch(device: torch.device, name: str, *args) -> None:
+    """:func:`call` with ``device`` as the current one and its current stream as the last argument."""
+    index = device.index
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return call(name, *args, _raw_stream(index))
+    if function(name)(*args, _raw_stream(index)) != 0:
+        call(name, *args, _raw_stream(index))            # (again, for the error: what failed launched nothing)
+
+
 def set_kernel_timing(enable: bool) -> None:
     load_library().xfh_set_kernel_timing(int(enable))
 
@@ -217,28 +235,27 @@ def check_gpu_inference(*tensors) -> None:
             raise ValueError("The 'hip' backend requires strided ROCm (cuda) tensors.")
 
 
-def check_gpu(*tensors) -> torch.device:
+def check_gpu(*tensors) -> None:
     """Device and layout guards of the operators that have a backward pass: strided ROCm tensors, all
-    on one device, which is returned."""
-    device = None
+    on one device."""
+    index = None
     for tensor in tensors:
         if tensor is None:
             continue
-        if tensor.device.type != "cuda" or tensor.layout != torch.strided:
+        if not tensor.is_cuda or tensor.layout is not torch.strided:
             raise ValueError("The 'hip' backend requires strided ROCm (cuda) tensors.")
-        if device is not None and tensor.device != device:
-            raise ValueError(f"The 'hip' backend requires tensors on one device, got {device} and {tensor.device}.")
-        device = tensor.device
-    return device
-
-
-def on_device(device: torch.device):
-    """Makes ``device`` the current one while a call is launched (nothing where it is already)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        if index is None:
+            index = tensor.get_device()
+        elif tensor.get_device() != index:
+            raise ValueError(f"The 'hip' backend requires tensors on one device, got cuda:{index} and {tensor.device}.")
 
 
 def needs_gradient(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def compute_dtype(x: torch.Tensor, *weights: torch.Tensor) -> torch.dtype:

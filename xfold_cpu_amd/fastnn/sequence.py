@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional, Union
 
 import torch
@@ -16,6 +17,10 @@ from . import native_hip as nh
 from . import ops
 
 _NO_STRIDES = (0, 0, 0)
+_CODES = {torch.float32: nh.F32, torch.bfloat16: nh.BF16}
+# nh.SequenceAttention as bytes: 14 addresses, 33 sizes and strides, scale, softcap, causal, dtype.
+_PACKED = struct.Struct("14Q33q2f2i")
+assert _PACKED.size == ctypes.sizeof(nh.SequenceAttention)
 
 
 def _rows(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
@@ -34,24 +39,32 @@ def _empty(like: torch.Tensor, heads: int, tokens: int, dim: int) -> torch.Tenso
     return torch.empty((batch, heads, tokens, dim), dtype=like.dtype, device=like.device)
 
 
+def _address(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _strides(t: Optional[torch.Tensor]) -> tuple:
+    return _NO_STRIDES if t is None else t.stride()[:3]
+
+
 def _call(name, q, k, v, out, lse, slopes, masks, options, dout=None, dq=None, dk=None, dv=None, dslopes=None):
     prefix, documents, lengths = masks
     causal, prefix_all, softcap, scale = options
     device = q.device
-    args = nh.SequenceAttention(
-        *(None if t is None else t.data_ptr()
-          for t in (q, k, v, out, lse, slopes, prefix, documents, lengths, dout, dq, dk, dv, dslopes)),
-        q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], v.shape[3],
+    batch, heads, queries, dim = q.shape
+    kv_heads, keys, value_dim = v.shape[1:]
+    args = _PACKED.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _address(lse), _address(slopes), _address(prefix),
+        _address(documents), _address(lengths), _address(dout), _address(dq), _address(dk), _address(dv),
+        _address(dslopes), batch, heads, kv_heads, queries, keys, dim, value_dim,
         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
-        *(s for t in (dout, dq, dk, dv) for s in (_NO_STRIDES if t is None else t.stride()[:3])),
-        0 if documents is None else documents.stride(0), prefix_all, scale, softcap, causal, nh.dtype_code(q.dtype))
-    at = ctypes.addressof(args)
-    with nh.on_device(device):
-        size = getattr(nh.load_library(), name + "_workspace_size")(at)
-        if size < 0:
-            nh.call(name, at, None, 0, None)             # (raises with what is wrong)
-        ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        nh.call(name, at, None if ws is None else ws.data_ptr(), size, nh.stream_of(device))
+        *_strides(dout), *_strides(dq), *_strides(dk), *_strides(dv),
+        0 if documents is None else documents.stride(0), prefix_all, scale, softcap, causal, _CODES[q.dtype])
+    size = nh.function(name + "_workspace_size")(args)
+    if size <= 0:                                        # (none needed, or arguments that the call refuses)
+        return nh.launch(device, name, args, None, 0)
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    nh.launch(device, name, args, ws.data_ptr(), size)
 
 
 def _forward(q, k, v, slopes, masks, options, keep):
@@ -73,20 +86,28 @@ class _SequenceAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        q, k, v, slopes, out, lse, *masks = ctx.saved_tensors
-        dout = _rows(dout, q.dtype)
-        dq, dk, dv = (_empty(t, *t.shape[1:]) for t in (q, k, v))
-        dslopes = torch.empty_like(slopes) if ctx.needs_input_grad[3] else None
-        _call("xfh_sequence_attention_backward", q, k, v, out, lse, slopes, masks, ctx.options, dout, dq, dk, dv, dslopes)
-        grads = [dq, dk, dv, dslopes]
-        for i, dtype in enumerate(ctx.dtypes):
-            if not ctx.needs_input_grad[i]:
-                grads[i] = None
-            elif grads[i].dtype != dtype:
-                grads[i] = ops.as_dtype(grads[i], dtype)
-        return (*grads, None, None, None, None, None)
+        # Gradients that are to be differentiated again get the node that refuses it.
+        return _backward_once(ctx, dout) if torch.is_grad_enabled() else _backward(ctx, dout)
+
+
+def _backward(ctx, dout):
+    q, k, v, slopes, out, lse, *masks = ctx.saved_tensors
+    dout = _rows(dout, q.dtype)
+    dq, dk, dv = (_empty(t, *t.shape[1:]) for t in (q, k, v))
+    needs = ctx.needs_input_grad
+    dslopes = torch.empty_like(slopes) if needs[3] else None
+    _call("xfh_sequence_attention_backward", q, k, v, out, lse, slopes, masks, ctx.options, dout, dq, dk, dv, dslopes)
+    grads = [dq, dk, dv, dslopes]
+    for i, dtype in enumerate(ctx.dtypes):
+        if not needs[i]:
+            grads[i] = None
+        elif grads[i].dtype != dtype:
+            grads[i] = ops.as_dtype(grads[i], dtype)
+    return (*grads, None, None, None, None, None)
+
+
+_backward_once = once_differentiable(_backward)
 
 
 def _integers(t, shape, what):
