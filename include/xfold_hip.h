@@ -459,6 +459,8 @@ typedef struct XfhSequenceAttention {
   const void *q, *k, *v;           /* [batch][heads][queries][dim], [batch][kv_heads][keys][dim], [..][keys][value_dim] */
   void *out;                       /* [batch][heads][queries][value_dim]; read by the backward pass */
   float *lse;                      /* fp32 [batch][heads][queries], for the backward pass; NULL: none */
+  void *out_low;                   /* bf16 [batch][heads][queries][value_dim], contiguous, or NULL: what out's
+                                    * rounding left out, which makes the backward pass more exact (bf16 only) */
   const float *slopes;             /* fp32 [heads], or NULL */
   const int32_t *prefix;           /* [batch], or NULL: prefix_all for every entry */
   const int32_t *documents;        /* [batch][keys] (row stride documents_stride), or NULL */

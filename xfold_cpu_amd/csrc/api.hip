@@ -955,7 +955,7 @@ static int sequence_args(const XfhSequenceAttention *p, SequenceArgs &a) {
   XFH_REQUIRE(p->causal || !(p->prefix || p->prefix_all), "sequence_attention: a prefix needs the causal mask");
   XFH_REQUIRE(std::isfinite(p->scale) && std::isfinite(p->softcap), "sequence_attention: scale and softcap must be finite");
   std::memset(&a, 0, sizeof(a));
-  a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.lse = p->lse; a.slopes = p->slopes;
+  a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.lse = p->lse; a.low = p->dtype == XFH_BF16 ? p->out_low : nullptr; a.slopes = p->slopes;
   a.prefix = p->prefix; a.documents = p->documents; a.lengths = p->lengths;
   a.dout = p->dout; a.dq = p->dq; a.dk = p->dk; a.dv = p->dv;
   a.documents_stride = p->documents_stride;

@@ -303,6 +303,7 @@ int norm_train_backward(const void *dy, int dy_dtype, int64_t lddy, const void *
 struct SequenceArgs {
   const void *q, *k, *v, *dout;
   void *out, *dq, *dk, *dv;
+  void *low;                 // [B][H][Nq][Dv] in bf16, out before its rounding less out, or null
   float *lse;                // [B][H][Nq], log2 of the sum of exp2 of the scores; +inf: no visible key
   float *delta;              // [B][H][Nq], dout . out
   float *slope_part;         // [H][B][Nq], or null

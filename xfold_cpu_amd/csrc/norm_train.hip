@@ -91,6 +91,36 @@ __device__ __forceinline__ void store_row(T *row, int C, int sub, const float (&
     }
   }
 }
+// The same as stored (to be converted when they are used: loads of a row to come must not be waited for).
+template <int LPR, int CH, bool VEC, typename T> struct RawRow {
+  T v[CH][8];
+  __device__ __forceinline__ void load(const T *row, int C, int sub) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if constexpr (VEC) {
+        const int at = column<LPR, VEC>(sub, c, 0);
+        typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+        constexpr int N = 8 * int(sizeof(T)) / 16;
+        u32x4 u[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = at < C ? reinterpret_cast<const u32x4 *>(row + at)[i] : u32x4{0, 0, 0, 0};
+        __builtin_memcpy(v[c], u, sizeof(u));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int at = column<LPR, VEC>(sub, c, e);
+          v[c][e] = at < C ? row[at] : T(0.f);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&o)[CH][8]) const {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[c][e] = to_f32(v[c][e]);
+  }
+};
 // A parameter vector in its own type (null: `absent` everywhere).
 template <int LPR, int CH, bool VEC>
 __device__ __forceinline__ void load_param(const void *p, int dtype, float absent, int C, int sub, float (&v)[CH][8]) {
@@ -168,6 +198,29 @@ __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
   if (a.stats && sub == 0) a.stats[row] = make_float2(mean, rstd);
 }
 
+// A row's dx (in g) from its x (in h; normalised on return) and dy (in g).
+template <int LPR, int CH>
+__device__ __forceinline__ void backward_row(float (&h)[CH][8], float (&g)[CH][8], const float (&w)[CH][8], float2 st, float inv,
+                                             float *red) {
+  float s[2] = {0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // Beyond the row's end h is -mean/sigma, but g, and with it every sum, is zero there.
+      h[c][e] = (h[c][e] - st.x) * st.y;
+      g[c][e] *= w[c][e];
+      s[0] += g[c][e];
+      s[1] += g[c][e] * h[c][e];
+    }
+  row_sums<LPR, 2>(s, red);
+  const float mg = s[0] * inv, mgh = s[1] * inv;
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[c][e] = st.y * (g[c][e] - mg - h[c][e] * mgh);
+}
+
 template <typename T, typename TO, int LPR, int CH, bool VEC>
 __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
   constexpr int R = kThreads / LPR;                     // rows at a time
@@ -181,33 +234,38 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[c][e] = db[c][e] = 0.f;
   const float inv = 1.0f / float(C);
-  for (int64_t row = int64_t(blockIdx.x) * R + group; row < a.rows; row += int64_t(gridDim.x) * R) {
-    float h[CH][8], g[CH][8];
-    load_row<LPR, CH, VEC>(static_cast<const T *>(a.x) + row * a.ldx, C, sub, h);
-    load_row<LPR, CH, VEC>(static_cast<const TO *>(a.dy) + row * a.lddy, C, sub, g);
-    const float2 st = a.stats[row];
-    float s[2] = {0.f, 0.f};
+  // The next row's loads are issued before the work on this one.
+  const int64_t step = int64_t(gridDim.x) * R;
+  RawRow<LPR, CH, VEC, T> xr;
+  RawRow<LPR, CH, VEC, TO> gr;
+  float2 next{};
+  const auto fetch = [&](int64_t row) {
+    xr.load(static_cast<const T *>(a.x) + row * a.ldx, C, sub);
+    gr.load(static_cast<const TO *>(a.dy) + row * a.lddy, C, sub);
+    next = a.stats[row];
+  };
+  int64_t row = int64_t(blockIdx.x) * R + group;
+  if (VEC && row < a.rows) fetch(row);
+  for (; row < a.rows; row += step) {
+    float h[CH][8], g[CH][8], d[CH][8];
+    if constexpr (!VEC) fetch(row);                      // (element by element it takes too many registers: 13.8 -> 17.7 us at 5003x769)
+    xr.get(h);
+    gr.get(g);
+    const float2 st = next;
+    if (VEC && row + step < a.rows) fetch(row + step);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[c][e] = g[c][e];
+    backward_row<LPR, CH>(h, g, w, st, inv, red);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        // Beyond the row's end h is -mean/sigma, but g, and with it every sum, is zero there.
-        h[c][e] = (h[c][e] - st.x) * st.y;
-        dw[c][e] += g[c][e] * h[c][e];
-        db[c][e] += g[c][e];
-        g[c][e] *= w[c][e];
-        s[0] += g[c][e];
-        s[1] += g[c][e] * h[c][e];
+        dw[c][e] += d[c][e] * h[c][e];
+        db[c][e] += d[c][e];
       }
-    row_sums<LPR, 2>(s, red);
-    const float mg = s[0] * inv, mgh = s[1] * inv;
-    if (a.dx) {
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) g[c][e] = st.y * (g[c][e] - mg - h[c][e] * mgh);
-      store_row<LPR, CH, VEC>(static_cast<T *>(a.dx) + row * C, C, sub, g);
-    }
+    if (a.dx) store_row<LPR, CH, VEC>(static_cast<T *>(a.dx) + row * C, C, sub, g);
   }
   if (!a.partial) return;
   float *pw = a.partial + int64_t(blockIdx.x) * C, *pb = pw + int64_t(gridDim.x) * C;
@@ -325,6 +383,61 @@ __global__ __launch_bounds__(16 * kSlices) void norm_params_kernel(const float *
   }
 }
 
+// The backward pass of few rows in one launch: workgroups [0, row_blocks) take the rows' dx, the others 64 columns of dw and
+// db each, over all rows (4 slices of them, a wavefront each; the four sums of a column are added in order).
+// Both read x and dy, of which there is little. 72 x 384 in fp32: 8.8 us of GPU time in the two launches
+// above, 4.6 in this one; it is the launch that counts, since the host bounds such calls.
+constexpr int64_t kFewRows = 256;
+template <typename T, typename TO, int LPR, int CH, bool VEC>
+__global__ __launch_bounds__(kThreads) void norm_backward_few_kernel(NormArgs a, int row_blocks, void *dw, int dw_dtype,
+                                                                     void *db, int db_dtype) {
+  constexpr int R = kThreads / LPR;
+  __shared__ float red[8];
+  __shared__ float2 part[4][64];
+  const int C = a.C;
+  if (int(blockIdx.x) >= row_blocks) {
+    const int slice = threadIdx.x >> 6, c = (int(blockIdx.x) - row_blocks) * 64 + (threadIdx.x & 63);
+    float sw = 0.f, sb = 0.f;
+    if (c < C) {
+#pragma unroll 4
+      for (int64_t row = slice; row < a.rows; row += 4) {
+        const float2 st = a.stats[row];
+        const float g = to_f32(static_cast<const TO *>(a.dy)[row * a.lddy + c]);
+        sw += g * ((to_f32(static_cast<const T *>(a.x)[row * a.ldx + c]) - st.x) * st.y);
+        sb += g;
+      }
+    }
+    part[slice][threadIdx.x & 63] = make_float2(sw, sb);
+    __syncthreads();
+    if (slice || c >= C) return;
+    float2 t = part[0][threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      t.x += part[i][threadIdx.x].x;
+      t.y += part[i][threadIdx.x].y;
+    }
+    if (dw) {
+      if (dw_dtype == XFH_F32) static_cast<float *>(dw)[c] = t.x;
+      else static_cast<bf16 *>(dw)[c] = bf16(t.x);
+    }
+    if (db) {
+      if (db_dtype == XFH_F32) static_cast<float *>(db)[c] = t.y;
+      else static_cast<bf16 *>(db)[c] = bf16(t.y);
+    }
+    return;
+  }
+  const int sub = threadIdx.x % LPR;
+  const int64_t row = int64_t(blockIdx.x) * R + threadIdx.x / LPR;
+  if (LPR < 256 && row >= a.rows) return;              // (LPR = 256: a workgroup per row)
+  float w[CH][8], h[CH][8], g[CH][8];
+  load_row<LPR, CH, VEC>(static_cast<const T *>(a.x) + row * a.ldx, C, sub, h);
+  load_row<LPR, CH, VEC>(static_cast<const TO *>(a.dy) + row * a.lddy, C, sub, g);
+  load_param<LPR, CH, VEC>(a.w, a.w_dtype, 1.f, C, sub, w);
+  const float2 st = a.stats[row];
+  backward_row<LPR, CH>(h, g, w, st, 1.0f / float(C), red);
+  store_row<LPR, CH, VEC>(static_cast<T *>(a.dx) + row * C, C, sub, g);
+}
+
 // Lanes and chunks of a row of C elements (chunks 0: wider than the registers hold).
 struct RowShape { int lpr, ch; };
 RowShape row_shape(int64_t C) {
@@ -340,14 +453,25 @@ RowShape row_shape(int64_t C) {
 int64_t backward_blocks(int64_t rows, int64_t C) {
   const RowShape s = row_shape(C);
   if (s.ch == 0) return rows < 64 ? rows : 64;
-  const int64_t groups = ceil_div(rows, kThreads / s.lpr);
-  return groups < 1024 ? groups : 1024;
+  // A row of sums per workgroup: with rows that take a whole workgroup, half as many.
+  const int64_t groups = ceil_div(rows, kThreads / s.lpr), most = 1024;
+  return groups < most ? groups : most;
 }
 
+// Where the few rows' launch writes dw and db itself.
+struct ParamGrads { void *dw; int dw_dtype; void *db; int db_dtype; };
+
+bool few_rows(const NormArgs &a, const ParamGrads *p) { return p && a.rows <= kFewRows && row_shape(a.C).ch > 0; }
+
 template <typename T, typename TO, int LPR, int CH>
-int launch_shape(const NormArgs &a, bool vec, bool backward, int64_t blocks, hipStream_t s) {
+int launch_shape(const NormArgs &a, bool vec, bool backward, int64_t blocks, const ParamGrads *p, hipStream_t s) {
   const dim3 grid{unsigned(blocks)};
-  if (backward) {
+  if (backward && few_rows(a, p)) {
+    const int row_blocks = a.dx ? int(ceil_div(a.rows, int64_t(kThreads / LPR))) : 0, col_blocks = int(ceil_div(int64_t(a.C), int64_t(64)));
+    const dim3 both{unsigned(row_blocks + col_blocks)};
+    if (vec) norm_backward_few_kernel<T, TO, LPR, CH, true><<<both, kThreads, 0, s>>>(a, row_blocks, p->dw, p->dw_dtype, p->db, p->db_dtype);
+    else norm_backward_few_kernel<T, TO, LPR, CH, false><<<both, kThreads, 0, s>>>(a, row_blocks, p->dw, p->dw_dtype, p->db, p->db_dtype);
+  } else if (backward) {
     if (vec) norm_backward_kernel<T, TO, LPR, CH, true><<<grid, kThreads, 0, s>>>(a);
     else norm_backward_kernel<T, TO, LPR, CH, false><<<grid, kThreads, 0, s>>>(a);
   } else {
@@ -357,7 +481,7 @@ int launch_shape(const NormArgs &a, bool vec, bool backward, int64_t blocks, hip
   return check_launch("layer_norm_train");
 }
 
-template <typename T, typename TO> int launch_typed(const NormArgs &a, bool backward, hipStream_t s) {
+template <typename T, typename TO> int launch_typed(const NormArgs &a, bool backward, const ParamGrads *p, hipStream_t s) {
   const RowShape shape = row_shape(a.C);
   const auto aligned = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   const bool vec = a.C % 8 == 0 && a.ldx % 8 == 0 && (!backward || a.lddy % 8 == 0) && aligned(a.x) && aligned(a.dy) &&
@@ -375,20 +499,20 @@ template <typename T, typename TO> int launch_typed(const NormArgs &a, bool back
     }
     return check_launch("layer_norm_train");
   }
-  if (shape.lpr == 16 && shape.ch == 1) return launch_shape<T, TO, 16, 1>(a, vec, backward, blocks, s);
-  if (shape.lpr == 16) return launch_shape<T, TO, 16, 2>(a, vec, backward, blocks, s);
-  if (shape.lpr == 64 && shape.ch == 1) return launch_shape<T, TO, 64, 1>(a, vec, backward, blocks, s);
-  if (shape.lpr == 64) return launch_shape<T, TO, 64, 2>(a, vec, backward, blocks, s);
-  if (shape.ch == 1) return launch_shape<T, TO, 256, 1>(a, vec, backward, blocks, s);
-  if (shape.ch == 2) return launch_shape<T, TO, 256, 2>(a, vec, backward, blocks, s);
-  if (shape.ch == 4) return launch_shape<T, TO, 256, 4>(a, vec, backward, blocks, s);
-  return launch_shape<T, TO, 256, 8>(a, vec, backward, blocks, s);
+  if (shape.lpr == 16 && shape.ch == 1) return launch_shape<T, TO, 16, 1>(a, vec, backward, blocks, p, s);
+  if (shape.lpr == 16) return launch_shape<T, TO, 16, 2>(a, vec, backward, blocks, p, s);
+  if (shape.lpr == 64 && shape.ch == 1) return launch_shape<T, TO, 64, 1>(a, vec, backward, blocks, p, s);
+  if (shape.lpr == 64) return launch_shape<T, TO, 64, 2>(a, vec, backward, blocks, p, s);
+  if (shape.ch == 1) return launch_shape<T, TO, 256, 1>(a, vec, backward, blocks, p, s);
+  if (shape.ch == 2) return launch_shape<T, TO, 256, 2>(a, vec, backward, blocks, p, s);
+  if (shape.ch == 4) return launch_shape<T, TO, 256, 4>(a, vec, backward, blocks, p, s);
+  return launch_shape<T, TO, 256, 8>(a, vec, backward, blocks, p, s);
 }
 
-int launch_norm(const NormArgs &a, int x_dtype, int y_dtype, bool backward, hipStream_t s) {
-  if (x_dtype == XFH_F32 && y_dtype == XFH_F32) return launch_typed<float, float>(a, backward, s);
-  if (x_dtype == XFH_BF16 && y_dtype == XFH_BF16) return launch_typed<bf16, bf16>(a, backward, s);
-  if (x_dtype == XFH_BF16 && y_dtype == XFH_F32) return launch_typed<bf16, float>(a, backward, s);
+int launch_norm(const NormArgs &a, int x_dtype, int y_dtype, bool backward, const ParamGrads *p, hipStream_t s) {
+  if (x_dtype == XFH_F32 && y_dtype == XFH_F32) return launch_typed<float, float>(a, backward, p, s);
+  if (x_dtype == XFH_BF16 && y_dtype == XFH_BF16) return launch_typed<bf16, bf16>(a, backward, p, s);
+  if (x_dtype == XFH_BF16 && y_dtype == XFH_F32) return launch_typed<bf16, float>(a, backward, p, s);
   return fail(XFH_EUNSUPPORTED, "layer_norm_train: x and y must be f32 and f32, bf16 and bf16, or bf16 and f32");
 }
 
@@ -400,10 +524,13 @@ int norm_train_forward(const void *x, int x_dtype, int64_t ldx, int64_t rows, in
   NormArgs a{};
   a.x = x; a.ldx = ldx; a.rows = rows; a.C = int(cols); a.w = w; a.w_dtype = w_dtype; a.b = b; a.b_dtype = b_dtype;
   a.eps = eps; a.y = y; a.stats = reinterpret_cast<float2 *>(stats);
-  return launch_norm(a, x_dtype, y_dtype, false, s);
+  return launch_norm(a, x_dtype, y_dtype, false, nullptr, s);
 }
 
-int64_t norm_train_backward_workspace(int64_t rows, int64_t cols) { return 2 * backward_blocks(rows, cols) * cols * 4; }
+int64_t norm_train_backward_workspace(int64_t rows, int64_t cols) {
+  if (rows <= kFewRows && row_shape(cols).ch > 0) return 0;
+  return 2 * backward_blocks(rows, cols) * cols * 4;
+}
 
 int norm_train_backward(const void *dy, int dy_dtype, int64_t lddy, const void *x, int x_dtype, int64_t ldx, int64_t rows,
                         int64_t cols, const void *w, int w_dtype, const float *stats, void *dx, void *dw, int dw_dtype,
@@ -413,8 +540,9 @@ int norm_train_backward(const void *dy, int dy_dtype, int64_t lddy, const void *
   a.x = x; a.ldx = ldx; a.dy = dy; a.lddy = lddy; a.rows = rows; a.C = int(cols); a.w = w; a.w_dtype = w_dtype;
   a.dx = dx; a.stats = reinterpret_cast<float2 *>(const_cast<float *>(stats));
   a.partial = dw || db ? partial : nullptr;
-  if (rows > 0 && (dx || a.partial)) XFH_TRY(launch_norm(a, x_dtype, dy_dtype, true, s));
-  if (!dw && !db) return XFH_OK;
+  const ParamGrads grads{dw, dw_dtype, db, db_dtype}, *params = dw || db ? &grads : nullptr;
+  if (rows > 0 && (dx || params)) XFH_TRY(launch_norm(a, x_dtype, dy_dtype, true, params, s));
+  if (!params || (rows > 0 && few_rows(a, params))) return XFH_OK;
   const int64_t blocks = backward_blocks(rows, cols);    // no rows: sums of nothing, zeros
   norm_params_kernel<<<dim3(unsigned(ceil_div(cols, int64_t(16))), 2), 16 * kSlices, 0, s>>>(partial, int(blocks), int(cols), dw,
                                                                                        dw_dtype, db, db_dtype);

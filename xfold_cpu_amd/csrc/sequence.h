@@ -74,7 +74,62 @@ template <> __device__ __forceinline__ float bend<bf16>(float t) {
   const float e = __builtin_amdgcn_exp2f(t * (2.0f * kLog2e));
   return 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
 }
+// A query's part of its slope's gradient: all = sum P, far = sum P |gap|, error = sum P (dP - delta), far_error =
+// sum P (dP - delta) |gap|. A query that sees nothing has none.
+__device__ __forceinline__ float slope_gradient(float all, float far, float error, float far_error) {
+  return all == 0.f ? 0.f : -(far_error - error * (far / all)) / all;
+}
+
 template <typename T> __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A tile of a walk: its number (-1: none is left), whether this wavefront's columns see any and all of it.
+struct Step { int tile; bool mine, whole; };
+
+// The walk over tiles [first, end), 64 of them at a time, one per lane. test(tile) says which of {the
+// workgroup needs it, the wavefront needs it, the wavefront's columns see it whole} hold.
+struct Needs { bool block, mine, whole; };
+struct Walk {
+  int first, end;
+  uint64_t need = 0, mine = 0, whole = 0;
+  __device__ __forceinline__ Walk(int f, int e) : first(f - 64), end(e) {}
+  template <class F> __device__ __forceinline__ Step next(F test) {
+    while (!need) {
+      first += 64;
+      if (first >= end) return {-1, false, false};
+      const int tile = first + int(threadIdx.x & 63);
+      Needs n{false, false, false};
+      if (tile < end) n = test(tile);
+      need = __ballot(n.block);
+      mine = __ballot(n.block && n.mine);
+      whole = __ballot(n.block && n.mine && n.whole);
+    }
+    const int bit = __builtin_ctzll(need);
+    need &= need - 1;
+    return {first + bit, bool((mine >> bit) & 1), bool((whole >> bit) & 1)};
+  }
+};
+
+// Bounds and documents of the keys that a run of queries sees.
+struct Span { int low, high; Range range; };
+__device__ __forceinline__ Span span_of(const SequenceArgs &a, const Place &p, int b, int i0, int i1) {
+  Span s{0, 0, Range{0x7fffffff, -1, 0, 0}};
+  if (i0 > i1) return s;
+  s.low = limit_of(a, p, i0);
+  s.high = limit_of(a, p, i1);
+  if (a.documents) s.range = query_range(a, p, b, i0, i1);
+  return s;
+}
+__device__ __forceinline__ Needs key_tile_needs(const SequenceArgs &a, int b, int tile, const Span &block, const Span &wave) {
+  const int k0 = tile * kTile;
+  Needs n{k0 < block.high, k0 < wave.high, k0 + kTile <= wave.low};
+  if (a.documents && n.block) {
+    const Range r = static_cast<const Range *>(a.ranges)[int64_t(b) * a.tiles + tile];
+    n.block = overlap(r, block.range);
+    n.mine = n.mine && overlap(r, wave.range);
+    n.whole = n.whole && same_document(r, wave.range);
+  }
+  return n;
+}
 
 }  // namespace seq
 }  // namespace xfh

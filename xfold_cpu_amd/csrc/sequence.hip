@@ -11,7 +11,8 @@
 // second ones up to a permutation of the 32 rows of a step; the A operand read applies the same. So no
 // score leaves its lane but for the sums over the four lanes of a column.
 //
-// Tiles that no owned token sees are skipped: a wavefront tests 64 tiles at a time, one per lane.
+// Tiles that no owned token sees are skipped: a wavefront tests 64 tiles at a time, one per lane. The next
+// tile's loads are issued before the work on the one in LDS.
 //
 // What a masked place holds does not matter: its score is replaced and its weight is 0, but in the
 // second products 0 times an infinity or a NaN of the other side is NaN. Such a sum cannot become
@@ -48,31 +49,59 @@ __global__ __launch_bounds__(256) void ranges_kernel(SequenceArgs a, Range *out)
 
 template <typename T> constexpr int pitch_pad() { return 16 / int(sizeof(T)); }
 
-// Rows [row0, row0 + 64) of a [rows][D] matrix into LDS, zero beyond its end and beyond D.
-template <typename T, int DP>
-__device__ __forceinline__ void load_tile(T *dst, const T *src, int64_t stride, int row0, int rows, int D, bool vec) {
-  constexpr int P = DP + pitch_pad<T>(), E = 16 / int(sizeof(T));
-  if (vec) {
-    typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
-    for (int i = threadIdx.x; i < kTile * DP / E; i += 256) {
-      const int r = i / (DP / E), c = (i % (DP / E)) * E;
-      u32x4 v = {0, 0, 0, 0};
-      if (row0 + r < rows && c < D) v = *reinterpret_cast<const u32x4 *>(src + int64_t(row0 + r) * stride + c);
-      *reinterpret_cast<u32x4 *>(dst + r * P + c) = v;
-    }
-  } else {
-    for (int i = threadIdx.x; i < kTile * DP; i += 256) {
-      const int r = i / DP, c = i % DP;
-      dst[r * P + c] = row0 + r < rows && c < D ? src[int64_t(row0 + r) * stride + c] : T(0.f);
+// Rows [row0, row0 + 64) of a [rows][D] matrix to LDS, zero beyond its end and beyond D, in two steps: `fetch` issues
+// the loads of the next tile before the work on this one, `put` stores them after it. Rows that are not
+// whole 16-byte pieces are read element by element by `put`.
+template <typename T, int DP> struct TileLoad {
+  typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+  static constexpr int P = DP + pitch_pad<T>(), E = 16 / int(sizeof(T)), N = kTile * DP / E / 256;
+  static_assert(N * 256 * E == kTile * DP, "whole pieces for each thread");
+  u32x4 v[N];
+  __device__ __forceinline__ void fetch(const T *src, int64_t stride, int row0, int rows, int D, bool vec) {
+    if (!vec) return;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = j * 256 + threadIdx.x, r = i / (DP / E), c = (i % (DP / E)) * E;
+      v[j] = u32x4{0, 0, 0, 0};
+      if (row0 + r < rows && c < D) v[j] = *reinterpret_cast<const u32x4 *>(src + int64_t(row0 + r) * stride + c);
     }
   }
-}
+  __device__ __forceinline__ void put(T *dst, const T *src, int64_t stride, int row0, int rows, int D, bool vec) const {
+    if (vec) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int i = j * 256 + threadIdx.x;
+        *reinterpret_cast<u32x4 *>(dst + i / (DP / E) * P + (i % (DP / E)) * E) = v[j];
+      }
+    } else {
+#pragma unroll 8
+      for (int i = threadIdx.x; i < kTile * DP; i += 256) {
+        const int r = i / DP, c = i % DP;
+        dst[r * P + c] = row0 + r < rows && c < D ? src[int64_t(row0 + r) * stride + c] : T(0.f);
+      }
+    }
+  }
+};
 // The owned token's row as B fragments: d = 32 step + 8 grp + 0..7.
 template <typename T, int DP>
-__device__ __forceinline__ void load_own(typename Frag<T>::type (&f)[DP / 32], const T *row, int D, bool valid, int grp) {
+__device__ __forceinline__ void load_own(typename Frag<T>::type (&f)[DP / 32], const T *row, int D, bool valid, int grp,
+                                         bool vec) {
 #pragma unroll
   for (int st = 0; st < DP / 32; ++st) {
-    T t[8];
+    __attribute__((aligned(16))) T t[8];
+    if (vec) {
+      typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+      constexpr int E = 16 / int(sizeof(T));
+#pragma unroll
+      for (int e = 0; e < 8; e += E) {
+        const int d = st * 32 + grp * 8 + e;
+        u32x4 v = {0, 0, 0, 0};
+        if (valid && d < D) v = *reinterpret_cast<const u32x4 *>(row + d);
+        __builtin_memcpy(t + e, &v, 16);
+      }
+      __builtin_memcpy(&f[st], t, sizeof(t));
+      continue;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int d = st * 32 + grp * 8 + e;
@@ -185,21 +214,6 @@ template <typename T> struct Scorer {
   }
 };
 
-// Which of the 64 tiles from tile `first` on a workgroup with queries [i0, i1] needs (bit = tile), and which
-// of these it sees whole.
-struct Visit { uint64_t need, whole; };
-__device__ __forceinline__ Visit visit_keys(const SequenceArgs &a, const Place &p, int b, int first, int low, int high,
-                                            const Range &mine) {
-  const int tile = first + int(threadIdx.x & 63), k0 = tile * kTile;
-  bool need = tile < a.tiles && k0 < high, whole = need && k0 + kTile <= low;
-  if (a.documents && need) {
-    const Range r = static_cast<const Range *>(a.ranges)[int64_t(b) * a.tiles + tile];
-    need = overlap(r, mine);
-    whole = whole && same_document(r, mine);
-  }
-  return {__ballot(need), __ballot(need && whole)};
-}
-
 struct Owner { int block, h, b; };
 // Query blocks from the last to the first (a causal mask gives the last the most work), heads fastest.
 __device__ __forceinline__ Owner owner_of(int blocks, int heads, int item) {
@@ -221,9 +235,10 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void forward_ker
   const T *kp = static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[1];
   const T *vp = static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[1];
   typename Frag<T>::type qf[DP / 32];
-  load_own<T, DP>(qf, static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1] + i * a.qs[2], a.D, valid, grp);
-  const int low = limit_of(a, place, i0), high = limit_of(a, place, i1);
-  const Range mine = a.documents ? query_range(a, place, b, i0, i1) : Range{};
+  load_own<T, DP>(qf, static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1] + i * a.qs[2], a.D, valid, grp, vec);
+  const Span span = span_of(a, place, b, i0, i1);
+  const int high = span.high;
+  const auto test = [&](int tile) { return key_tile_needs(a, b, tile, span, span); };
   const Scorer<T> score(a, h);
 
   f32x4 o[DP / 16];
@@ -233,17 +248,27 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void forward_ker
     l = 0.f;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int first = 0; first * kTile < high; first += 64) {
-      Visit visit = visit_keys(a, place, b, first, low, high, mine);
-      while (visit.need) {
-        const int bit = __builtin_ctzll(visit.need), k0 = (first + bit) * kTile;
-        const bool whole = (visit.whole >> bit) & 1;
-        visit.need &= visit.need - 1;
+    Walk walk(0, (high + kTile - 1) / kTile);
+    Step now = walk.next(test);
+    TileLoad<T, DP> kt, vt;
+    int id = -1;
+    const auto fetch = [&](int k0) {
+      kt.fetch(kp, a.ks[2], k0, place.n, a.D, vec);
+      vt.fetch(vp, a.vs[2], k0, place.n, a.Dv, vec);
+      if (a.documents && tid < kTile) id = k0 + tid < place.n ? a.documents[int64_t(b) * a.documents_stride + k0 + tid] : -1;
+    };
+    if (now.tile >= 0) fetch(now.tile * kTile);
+    {
+      while (now.tile >= 0) {
+        const int k0 = now.tile * kTile;
+        const bool whole = now.whole;
         __syncthreads();
-        load_tile<T, DP>(ks, kp, a.ks[2], k0, place.n, a.D, vec);
-        load_tile<T, DP>(vs, vp, a.vs[2], k0, place.n, a.Dv, vec);
-        if (a.documents && tid < kTile) ids[tid] = k0 + tid < place.n ? a.documents[int64_t(b) * a.documents_stride + k0 + tid] : -1;
+        kt.put(ks, kp, a.ks[2], k0, place.n, a.D, vec);
+        vt.put(vs, vp, a.vs[2], k0, place.n, a.Dv, vec);
+        if (tid < kTile) ids[tid] = id;
         __syncthreads();
+        now = walk.next(test);
+        if (now.tile >= 0) fetch(now.tile * kTile);
         f32x4 s[4];
         tile_product<T, DP>(ks, qf, s);
         float w[4][4];
@@ -295,14 +320,20 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void forward_ker
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int d = t * 16 + grp * 4 + e;
-      if (d < a.Dv) op[d] = from_f32<T>(o[t][e] * inv);
+      if (d < a.Dv) {
+        const float x = o[t][e] * inv;
+        const T r = from_f32<T>(x);
+        op[d] = r;
+        if (a.low) static_cast<bf16 *>(a.low)[((int64_t(b) * a.H + h) * a.Nq + i) * a.Dv + d] = bf16(x - to_f32(r));
+      }
     }
   if (a.lse && grp == 0) a.lse[(int64_t(b) * a.H + h) * a.Nq + i] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
 // dq of 64 queries, their delta = dout . out (for dk and dv), and the slopes' part of each query,
 //   - sum_j P (dP - sum P dP) |gap| = - (sum_j P (dP - delta) |gap| - (sum_j P (dP - delta)) (sum_j P |gap|)),
-// in fp32 from unrounded values: delta, which has the output's rounding in it, drops out.
+// in fp32 from unrounded values: delta, which has the output's rounding in it, drops out, and so does
+// what the row's P are off by together, since each sum is divided by theirs.
 template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(SequenceArgs a, int blocks, bool vec) {
   constexpr int P = DP + pitch_pad<T>();
   __shared__ __attribute__((aligned(16))) T ks[kTile * P], vs[kTile * P];
@@ -317,39 +348,51 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
   const T *kp = static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[1];
   const T *vp = static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[1];
   typename Frag<T>::type qf[DP / 32], gf[DP / 32];
-  load_own<T, DP>(qf, static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1] + i * a.qs[2], a.D, valid, grp);
+  load_own<T, DP>(qf, static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1] + i * a.qs[2], a.D, valid, grp, vec);
   const T *gp = static_cast<const T *>(a.dout) + b * a.gs[0] + h * a.gs[1] + i * a.gs[2];
   const T *op = static_cast<const T *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2];
-  load_own<T, DP>(gf, gp, a.Dv, valid, grp);
+  load_own<T, DP>(gf, gp, a.Dv, valid, grp, vec);
   float delta = 0.f;
+  const int64_t at = (int64_t(b) * a.H + h) * a.Nq + i;
+  const bf16 *low = a.low ? static_cast<const bf16 *>(a.low) + at * a.Dv : nullptr;
   if (valid)
     for (int d0 = grp * 8; d0 < a.Dv; d0 += 32)
-      for (int d = d0; d < min(d0 + 8, a.Dv); ++d) delta += to_f32(gp[d]) * to_f32(op[d]);
+      for (int d = d0; d < min(d0 + 8, a.Dv); ++d) delta += to_f32(gp[d]) * (to_f32(op[d]) + (low ? to_f32(low[d]) : 0.f));
   delta = column_sum(delta);
-  const int64_t at = (int64_t(b) * a.H + h) * a.Nq + i;
   const float lse = valid ? a.lse[at] : INFINITY;
   if (valid && grp == 0) a.delta[at] = delta;
-  const int low = limit_of(a, place, i0), high = limit_of(a, place, i1);
-  const Range mine = a.documents ? query_range(a, place, b, i0, i1) : Range{};
+  const Span span = span_of(a, place, b, i0, i1);
+  const int high = span.high;
+  const auto test = [&](int tile) { return key_tile_needs(a, b, tile, span, span); };
   const Scorer<T> score(a, h);
 
   f32x4 dq[DP / 16];
-  float far, error, far_error;
+  float all, far, error, far_error;
   for (int strict = 0; strict < 2; ++strict) {
-    far = error = far_error = 0.f;
+    all = far = error = far_error = 0.f;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) dq[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int first = 0; first * kTile < high; first += 64) {
-      Visit visit = visit_keys(a, place, b, first, low, high, mine);
-      while (visit.need) {
-        const int bit = __builtin_ctzll(visit.need), k0 = (first + bit) * kTile;
-        const bool whole = (visit.whole >> bit) & 1;
-        visit.need &= visit.need - 1;
+    Walk walk(0, (high + kTile - 1) / kTile);
+    Step now = walk.next(test);
+    TileLoad<T, DP> kt, vt;
+    int id = -1;
+    const auto fetch = [&](int k0) {
+      kt.fetch(kp, a.ks[2], k0, place.n, a.D, vec);
+      vt.fetch(vp, a.vs[2], k0, place.n, a.Dv, vec);
+      if (a.documents && tid < kTile) id = k0 + tid < place.n ? a.documents[int64_t(b) * a.documents_stride + k0 + tid] : -1;
+    };
+    if (now.tile >= 0) fetch(now.tile * kTile);
+    {
+      while (now.tile >= 0) {
+        const int k0 = now.tile * kTile;
+        const bool whole = now.whole;
         __syncthreads();
-        load_tile<T, DP>(ks, kp, a.ks[2], k0, place.n, a.D, vec);
-        load_tile<T, DP>(vs, vp, a.vs[2], k0, place.n, a.Dv, vec);
-        if (a.documents && tid < kTile) ids[tid] = k0 + tid < place.n ? a.documents[int64_t(b) * a.documents_stride + k0 + tid] : -1;
+        kt.put(ks, kp, a.ks[2], k0, place.n, a.D, vec);
+        vt.put(vs, vp, a.vs[2], k0, place.n, a.Dv, vec);
+        if (tid < kTile) ids[tid] = id;
         __syncthreads();
+        now = walk.next(test);
+        if (now.tile >= 0) fetch(now.tile * kTile);
         f32x4 s[4], dp[4];
         tile_product<T, DP>(ks, qf, s);
         tile_product<T, DP>(vs, gf, dp);
@@ -369,6 +412,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
             seen |= see ? 1u << (4 * kt + e) : 0u;
             if (a.slope_part && see) {
               const float gap = fabsf(float(row.pos - key));
+              all += p;
               far += p * gap;
               error += ds;
               far_error += ds * gap;
@@ -395,10 +439,11 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
       }
   }
   if (a.slope_part) {
+    all = column_sum(all);
     far = column_sum(far);
     error = column_sum(error);
     far_error = column_sum(far_error);
-    if (valid && grp == 0) a.slope_part[(int64_t(h) * a.B + b) * a.Nq + i] = -(far_error - error * far);
+    if (valid && grp == 0) a.slope_part[(int64_t(h) * a.B + b) * a.Nq + i] = slope_gradient(all, far, error, far_error);
   }
 }
 
@@ -415,8 +460,8 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dkv_kernel(
   const int k0 = block * kTile, key = k0 + wave * 16 + col;
   const bool valid = key < place.n;
   typename Frag<T>::type kf[DP / 32], vf[DP / 32];
-  load_own<T, DP>(kf, static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[1] + key * a.ks[2], a.D, valid, grp);
-  load_own<T, DP>(vf, static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[1] + key * a.vs[2], a.Dv, valid, grp);
+  load_own<T, DP>(kf, static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[1] + key * a.ks[2], a.D, valid, grp, vec);
+  load_own<T, DP>(vf, static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[1] + key * a.vs[2], a.Dv, valid, grp, vec);
   int id = 0;
   Range mine{};
   if (a.documents) {
@@ -435,30 +480,47 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dkv_kernel(
       const T *gp = static_cast<const T *>(a.dout) + b * a.gs[0] + h * a.gs[1];
       const Scorer<T> score(a, h);
       const int64_t at = (int64_t(b) * a.H + h) * a.Nq;
-      for (int first = 0; first < qtiles; first += 64) {
-        const int tile = first + lane, r0 = tile * kTile, r1 = min(r0 + kTile, a.Nq) - 1;
-        bool need = tile < qtiles && limit_of(a, place, r1) > k0, whole = need && limit_of(a, place, r0) >= k0 + kTile;
-        if (a.documents && need) {
+      const auto test = [&](int tile) {
+        const int r0 = tile * kTile, r1 = min(r0 + kTile, a.Nq) - 1;
+        Needs n{limit_of(a, place, r1) > k0, true, r0 + kTile <= a.Nq && limit_of(a, place, r0) >= k0 + kTile};
+        if (a.documents && n.block) {
           const Range r = query_range(a, place, b, r0, r1);
-          need = overlap(r, mine);
-          whole = whole && same_document(r, mine);
+          n.block = overlap(r, mine);
+          n.whole = n.whole && same_document(r, mine);
         }
-        uint64_t todo = __ballot(need);
-        const uint64_t wholes = __ballot(need && whole && r0 + kTile <= a.Nq);
-        while (todo) {
-          const int bit = __builtin_ctzll(todo), i0 = (first + bit) * kTile;
-          const bool all = (wholes >> bit) & 1;
-          todo &= todo - 1;
+        return n;
+      };
+      Walk walk(0, qtiles);
+      Step now = walk.next(test);
+      TileLoad<T, DP> qt, gt;
+      Row next_row{};
+      float next_lse = INFINITY, next_delta = 0.f;
+      const auto fetch = [&](int i0) {
+        qt.fetch(qp, a.qs[2], i0, a.Nq, a.D, vec);
+        gt.fetch(gp, a.gs[2], i0, a.Nq, a.Dv, vec);
+        if (tid < kTile) {
+          const int i = i0 + tid;
+          next_row = row_of(a, place, b, i);
+          next_lse = i < a.Nq ? a.lse[at + i] : INFINITY;
+          next_delta = i < a.Nq ? a.delta[at + i] : 0.f;
+        }
+      };
+      if (now.tile >= 0) fetch(now.tile * kTile);
+      {
+        while (now.tile >= 0) {
+          const int i0 = now.tile * kTile;
+          const bool all = now.whole;
           __syncthreads();
-          load_tile<T, DP>(qs, qp, a.qs[2], i0, a.Nq, a.D, vec);
-          load_tile<T, DP>(gs, gp, a.gs[2], i0, a.Nq, a.Dv, vec);
+          qt.put(qs, qp, a.qs[2], i0, a.Nq, a.D, vec);
+          gt.put(gs, gp, a.gs[2], i0, a.Nq, a.Dv, vec);
           if (tid < kTile) {
-            const int i = i0 + tid;
-            rows[tid] = row_of(a, place, b, i);
-            lses[tid] = i < a.Nq ? a.lse[at + i] : INFINITY;
-            deltas[tid] = i < a.Nq ? a.delta[at + i] : 0.f;
+            rows[tid] = next_row;
+            lses[tid] = next_lse;
+            deltas[tid] = next_delta;
           }
           __syncthreads();
+          now = walk.next(test);
+          if (now.tile >= 0) fetch(now.tile * kTile);
           f32x4 s[4], dp[4];
           tile_product<T, DP>(qs, kf, s);
           tile_product<T, DP>(gs, vf, dp);
@@ -527,7 +589,7 @@ template <typename T> bool vector_rows(std::initializer_list<std::pair<const voi
 
 template <typename T, int DP> int launch_forward(const SequenceArgs &a, hipStream_t s) {
   const int64_t blocks = ceil_div(a.Nq, int64_t(kTile));
-  const bool vec = vector_rows<T>({{a.k, a.ks}}, a.D) && vector_rows<T>({{a.v, a.vs}}, a.Dv);
+  const bool vec = vector_rows<T>({{a.q, a.qs}, {a.k, a.ks}}, a.D) && vector_rows<T>({{a.v, a.vs}}, a.Dv);
   forward_kernel<T, DP><<<dim3(unsigned(blocks * a.H * a.B)), 256, 0, s>>>(a, int(blocks), vec);
   return check_launch("sequence_attention");
 }

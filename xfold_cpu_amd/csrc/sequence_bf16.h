@@ -220,55 +220,6 @@ template <int MODE> struct Score {
   __device__ __forceinline__ float in_log2(float w) const { return RAW ? w * unit : w; }
 };
 
-// A tile of a walk: its number (-1: none is left), whether this wavefront's columns see any and all of it.
-struct Step { int tile; bool mine, whole; };
-
-// The walk over tiles [first, end), 64 of them at a time, one per lane. test(tile) says which of {the
-// workgroup needs it, the wavefront needs it, the wavefront's columns see it whole} hold.
-struct Needs { bool block, mine, whole; };
-struct Walk {
-  int first, end;
-  uint64_t need = 0, mine = 0, whole = 0;
-  __device__ __forceinline__ Walk(int f, int e) : first(f - 64), end(e) {}
-  template <class F> __device__ __forceinline__ Step next(F test) {
-    while (!need) {
-      first += 64;
-      if (first >= end) return {-1, false, false};
-      const int tile = first + int(threadIdx.x & 63);
-      Needs n{false, false, false};
-      if (tile < end) n = test(tile);
-      need = __ballot(n.block);
-      mine = __ballot(n.block && n.mine);
-      whole = __ballot(n.block && n.mine && n.whole);
-    }
-    const int bit = __builtin_ctzll(need);
-    need &= need - 1;
-    return {first + bit, bool((mine >> bit) & 1), bool((whole >> bit) & 1)};
-  }
-};
-
-// Bounds and documents of the keys that a run of queries sees.
-struct Span { int low, high; Range range; };
-__device__ __forceinline__ Span span_of(const SequenceArgs &a, const Place &p, int b, int i0, int i1) {
-  Span s{0, 0, Range{0x7fffffff, -1, 0, 0}};
-  if (i0 > i1) return s;
-  s.low = limit_of(a, p, i0);
-  s.high = limit_of(a, p, i1);
-  if (a.documents) s.range = query_range(a, p, b, i0, i1);
-  return s;
-}
-__device__ __forceinline__ Needs key_tile_needs(const SequenceArgs &a, int b, int tile, const Span &block, const Span &wave) {
-  const int k0 = tile * kTile;
-  Needs n{k0 < block.high, k0 < wave.high, k0 + kTile <= wave.low};
-  if (a.documents && n.block) {
-    const Range r = static_cast<const Range *>(a.ranges)[int64_t(b) * a.tiles + tile];
-    n.block = overlap(r, block.range);
-    n.mine = n.mine && overlap(r, wave.range);
-    n.whole = n.whole && same_document(r, wave.range);
-  }
-  return n;
-}
-
 // What a wavefront looks up to hide pairs: bounds and documents of the rows of a tile, in LDS of its own (a
 // lane works out one row; the 16 rows of a lane's registers are then eight 16-byte reads).
 struct Marks { int limit[kTile], document[kTile]; };
@@ -319,7 +270,8 @@ template <int T> __device__ __forceinline__ bool any_bad(const f32x16 (&o)[T]) {
 
 // A column's result: dims 32 t + 8 j + 4 half .. + 3, four at a time.
 template <int T>
-__device__ __forceinline__ void store_column(bf16 *out, int dim, const f32x16 (&o)[T], float scale, int half) {
+__device__ __forceinline__ void store_column(bf16 *out, int dim, const f32x16 (&o)[T], float scale, int half,
+                                             bf16 *low = nullptr) {
 #pragma unroll
   for (int t = 0; t < T; ++t)
 #pragma unroll
@@ -330,6 +282,12 @@ __device__ __forceinline__ void store_column(bf16 *out, int dim, const f32x16 (&
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = static_cast<bf16>(o[t][4 * j + e] * scale);
         *reinterpret_cast<bf16x4 *>(out + d) = v;
+        if (low) {
+          bf16x4 u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[e] = static_cast<bf16>(o[t][4 * j + e] * scale - static_cast<float>(v[e]));
+          *reinterpret_cast<bf16x4 *>(low + d) = u;
+        }
       }
     }
 }

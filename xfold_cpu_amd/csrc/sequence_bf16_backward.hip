@@ -12,7 +12,7 @@ using namespace seq;
 
 // ------------------------------------------------------------------------------ dq
 
-struct SlopeSums { float far, error, far_error; };       // sum P |gap|, sum P (dP - delta), sum P (dP - delta) |gap|
+struct SlopeSums { float all, far, error, far_error; };  // as slope_gradient takes them
 
 template <class D, int MODE, bool STRICT>
 __device__ __forceinline__ void dq_walk(const SequenceArgs &a, const Lane<D> &ln, bf16 *stage0, bf16 *stage1,
@@ -21,7 +21,7 @@ __device__ __forceinline__ void dq_walk(const SequenceArgs &a, const Lane<D> &ln
                                         const Span &block, const Span &wave, const Row &row, Marks &marks, float lse,
                                         float delta, f32x16 (&dq)[D::DT], SlopeSums &sums) {
   constexpr int TILE = kTile * D::DL;
-  sums = SlopeSums{0.f, 0.f, 0.f};
+  sums = SlopeSums{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int t = 0; t < D::DT; ++t) dq[t] = zeros16();
   const auto test = [&](int tile) { return key_tile_needs(a, b, tile, block, wave); };
@@ -57,6 +57,7 @@ __device__ __forceinline__ void dq_walk(const SequenceArgs &a, const Lane<D> &ln
         if constexpr (Score<MODE>::SLOPE) {
           const float away = fabsf(gap - float(row_of_register(r)));
           if (a.slope_part) {
+            sums.all += p;
             sums.far = __builtin_fmaf(p, away, sums.far);
             sums.error += ds;
             sums.far_error = __builtin_fmaf(ds, away, sums.far_error);
@@ -124,12 +125,14 @@ __global__ __launch_bounds__(256, 2) void dq_bf16_kernel(SequenceArgs a, int blo
   const int64_t at = (int64_t(b) * a.H + h) * a.Nq + i;
   float delta = 0.f;
   {
-    bf16x8 of[D::KS];
+    bf16x8 of[D::KS], lf[D::KS] = {};
     own_row<D>(of, static_cast<const bf16 *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2], a.Dv, valid, ln.half);
+    if (a.low) own_row<D>(lf, static_cast<const bf16 *>(a.low) + at * a.Dv, a.Dv, valid, ln.half);
 #pragma unroll
     for (int ks = 0; ks < D::KS; ++ks)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(static_cast<float>(of[ks][e]), static_cast<float>(gf[ks][e]), delta);
+      for (int e = 0; e < 8; ++e)
+        delta = __builtin_fmaf(static_cast<float>(of[ks][e]) + static_cast<float>(lf[ks][e]), static_cast<float>(gf[ks][e]), delta);
   }
   delta += other_half(delta);
   const float lse = valid ? a.lse[at] : INFINITY;
@@ -146,11 +149,12 @@ __global__ __launch_bounds__(256, 2) void dq_bf16_kernel(SequenceArgs a, int blo
     store_column(static_cast<bf16 *>(a.dq) + b * a.dqs[0] + h * a.dqs[1] + i * a.dqs[2], a.D, dq, a.scale, ln.half);
   if constexpr (Score<MODE>::SLOPE) {
     if (!a.slope_part) return;
+    sums.all += other_half(sums.all);
     sums.far += other_half(sums.far);
     sums.error += other_half(sums.error);
     sums.far_error += other_half(sums.far_error);
     // One part per query and head: slope_part [H][B][Nq].
-    if (valid && ln.half == 0) a.slope_part[(int64_t(h) * a.B + b) * a.Nq + i] = -(sums.far_error - sums.error * sums.far);
+    if (valid && ln.half == 0) a.slope_part[(int64_t(h) * a.B + b) * a.Nq + i] = slope_gradient(sums.all, sums.far, sums.error, sums.far_error);
   }
 }
 
@@ -430,7 +434,7 @@ Splits dkv_splits(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk) {
 }  // namespace
 
 bool sequence_bf16_backward_fits(const SequenceArgs &a) {
-  return sequence_bf16_forward_fits(a) && rows_fit(a.out, a.os, a.Dv, 8) && rows_fit(a.dout, a.gs, a.Dv, 8) &&
+  return sequence_bf16_forward_fits(a) && rows_fit(a.out, a.os, a.Dv, 8) && rows_fit(a.dout, a.gs, a.Dv, 8) && reinterpret_cast<uintptr_t>(a.low) % 16 == 0 &&
          rows_fit(a.dq, a.dqs, a.D, 4) && rows_fit(a.dk, a.dks, a.D, 4) && rows_fit(a.dv, a.dvs, a.Dv, 4);
 }
 

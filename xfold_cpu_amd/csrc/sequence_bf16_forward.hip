@@ -177,7 +177,8 @@ __global__ __launch_bounds__(256, 2) void forward_bf16_kernel(SequenceArgs a, in
       }
     return;
   }
-  store_column(static_cast<bf16 *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2], a.Dv, o, l == 0.f ? 0.f : 1.0f / l, ln.half);
+  store_column(static_cast<bf16 *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2], a.Dv, o, l == 0.f ? 0.f : 1.0f / l, ln.half,
+               a.low ? static_cast<bf16 *>(a.low) + ((int64_t(b) * a.H + h) * a.Nq + i) * a.Dv : nullptr);
   if (a.lse && ln.half == 0) a.lse[(int64_t(b) * a.H + h) * a.Nq + i] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -290,7 +291,10 @@ __global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, int 
       parts.o[p * a.Dv + d] = value;
       if (d == 0) parts.ml[p] = make_float2(top, sum);
     } else {
-      static_cast<bf16 *>(a.out)[b * a.os[0] + head * a.os[1] + query * a.os[2] + d] = bf16(sum == 0.f ? 0.f : value / sum);
+      const float x = sum == 0.f ? 0.f : value / sum;
+      const bf16 r = bf16(x);
+      static_cast<bf16 *>(a.out)[b * a.os[0] + head * a.os[1] + query * a.os[2] + d] = r;
+      if (a.low) static_cast<bf16 *>(a.low)[((int64_t(b) * a.H + head) * a.Nq + query) * a.Dv + d] = bf16(x - static_cast<float>(r));
       if (a.lse && d == 0)
         a.lse[(int64_t(b) * a.H + head) * a.Nq + query] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
     }
@@ -322,6 +326,12 @@ __global__ __launch_bounds__(256) void join_kernel(SequenceArgs a, Parts parts) 
 #pragma unroll
   for (int e = 0; e < 4; ++e) r[e] = static_cast<bf16>(v[e] * inv);
   *reinterpret_cast<bf16x4 *>(out) = r;
+  if (a.low) {
+    bf16x4 u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = static_cast<bf16>(v[e] * inv - static_cast<float>(r[e]));
+    *reinterpret_cast<bf16x4 *>(static_cast<bf16 *>(a.low) + ((int64_t(b) * a.H + h) * a.Nq + i) * a.Dv + d) = u;
+  }
   if (a.lse && d == 0) a.lse[(int64_t(b) * a.H + h) * a.Nq + i] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
@@ -329,7 +339,7 @@ __global__ __launch_bounds__(256) void join_kernel(SequenceArgs a, Parts parts) 
 
 bool sequence_bf16_forward_fits(const SequenceArgs &a) {
   return rows_fit(a.q, a.qs, a.D, 8) && rows_fit(a.k, a.ks, a.D, 8) && rows_fit(a.v, a.vs, a.Dv, 8) && rows_fit(a.out, a.os, a.Dv, 4) &&
-         int64_t(a.H / a.Hk) * a.Nq < (int64_t(1) << 31) - 256;
+         reinterpret_cast<uintptr_t>(a.low) % 8 == 0 && int64_t(a.H / a.Hk) * a.Nq < (int64_t(1) << 31) - 256;
 }
 
 int sequence_splits(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk) {

@@ -42,29 +42,37 @@ def _forward(x, cols, weight, bias, eps, out_dtype, keep):
     stats = torch.empty((rows, 2), dtype=torch.float32, device=device) if keep else None
     nh.launch(device, "xfh_layer_norm_train", x.data_ptr(), _CODES[x.dtype], stride, rows, cols, *_arg(weight),
               *_arg(bias), eps, y.data_ptr(), _CODES[out_dtype], None if stats is None else stats.data_ptr())
-    return x, y, stats
+    return x, y, stats, stride
 
 
 def _backward(ctx, dy):
+    # (Runs in a thread of autograd's, where Python is slow: what is known before is in ctx.call.)
     x, weight, stats = ctx.saved_tensors
-    need_x, need_w, need_b = ctx.needs_input_grad[:3]
-    cols, out_dtype, bias = ctx.call
-    device = x.device
-    if dy.dtype != out_dtype:
+    need_x, need_w, need_b, *_ = ctx.needs_input_grad
+    cols, rows, x_code, x_stride, out_dtype, out_code, bias, size = ctx.call
+    if dy.dtype is not out_dtype:
         dy = dy.to(out_dtype)
-    dy, dy_stride = _rows(dy, cols)
-    x, x_stride = _rows(x, cols)
-    rows = stats.shape[0]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
-    dw = torch.empty_like(weight) if need_w else None
-    db = torch.empty(bias[0], dtype=bias[1], device=device) if need_b else None
-    ws, size = None, 0
-    if need_w or need_b:
-        size = nh.function("xfh_layer_norm_backward_workspace_size")(rows, cols)
-        ws = torch.empty(size, dtype=torch.uint8, device=device)
-    nh.launch(device, "xfh_layer_norm_backward", dy.data_ptr(), _CODES[out_dtype], dy_stride, x.data_ptr(),
-              _CODES[x.dtype], x_stride, rows, cols, *_arg(weight), stats.data_ptr(),
-              None if dx is None else dx.data_ptr(), *_arg(dw), *_arg(db), None if ws is None else ws.data_ptr(), size)
+    dy_stride = cols
+    if not dy.is_contiguous():
+        dy, dy_stride = _rows(dy, cols)
+    dx = dw = db = None
+    dx_at = dw_at = db_at = ws_at = None
+    dw_code = db_code = nh.F32
+    if need_x:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx_at = dx.data_ptr()
+    if need_w:
+        dw = torch.empty_like(weight)
+        dw_at, dw_code = dw.data_ptr(), _CODES[dw.dtype]
+    if need_b:
+        db = torch.empty(bias[0], dtype=bias[1], device=x.device)
+        db_at, db_code = db.data_ptr(), _CODES[bias[1]]
+    if size and (need_w or need_b):
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        ws_at = ws.data_ptr()
+    w_at, w_code = _arg(weight)
+    nh.launch(x.device, "xfh_layer_norm_backward", dy.data_ptr(), out_code, dy_stride, x.data_ptr(), x_code, x_stride, rows,
+              cols, w_at, w_code, stats.data_ptr(), dx_at, dw_at, dw_code, db_at, db_code, ws_at, size)
     return dx, dw, db, None, None, None
 
 
@@ -75,9 +83,12 @@ class _TrainableLayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, cols, eps, out_dtype):
         w = None if weight is None else weight.contiguous()
-        x, y, stats = _forward(x, cols, w, None if bias is None else bias.contiguous(), eps, out_dtype, True)
+        x, y, stats, stride = _forward(x, cols, w, None if bias is None else bias.contiguous(), eps, out_dtype, True)
+        rows = stats.shape[0]
         ctx.save_for_backward(x, w, stats)
-        ctx.call = cols, out_dtype, None if bias is None else (bias.shape, bias.dtype)
+        ctx.call = (cols, rows, _CODES[x.dtype], stride, out_dtype, _CODES[out_dtype],
+                    None if bias is None else (bias.shape, bias.dtype),
+                    nh.function("xfh_layer_norm_backward_workspace_size")(rows, cols))
         return y
 
     @staticmethod

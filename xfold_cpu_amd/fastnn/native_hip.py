@@ -146,7 +146,7 @@ class DiffusionBlock(ctypes.Structure):
 class SequenceAttention(ctypes.Structure):
     """``XfhSequenceAttention`` of include/xfold_hip.h, its strides one by one."""
     _fields_ = [(name, ctypes.c_void_p) for name in
-                ("q", "k", "v", "out", "lse", "slopes", "prefix", "documents", "lengths", "dout", "dq", "dk", "dv",
+                ("q", "k", "v", "out", "lse", "out_low", "slopes", "prefix", "documents", "lengths", "dout", "dq", "dk", "dv",
                  "dslopes")] + [
                (name, ctypes.c_int64) for name in
                ("batch", "heads", "kv_heads", "queries", "keys", "dim", "value_dim",

@@ -18,8 +18,8 @@ from . import ops
 
 _NO_STRIDES = (0, 0, 0)
 _CODES = {torch.float32: nh.F32, torch.bfloat16: nh.BF16}
-# nh.SequenceAttention as bytes: 14 addresses, 33 sizes and strides, scale, softcap, causal, dtype.
-_PACKED = struct.Struct("14Q33q2f2i")
+# nh.SequenceAttention as bytes: 15 addresses, 33 sizes and strides, scale, softcap, causal, dtype.
+_PACKED = struct.Struct("15Q33q2f2i")
 assert _PACKED.size == ctypes.sizeof(nh.SequenceAttention)
 
 
@@ -47,14 +47,14 @@ def _strides(t: Optional[torch.Tensor]) -> tuple:
     return _NO_STRIDES if t is None else t.stride()[:3]
 
 
-def _call(name, q, k, v, out, lse, slopes, masks, options, dout=None, dq=None, dk=None, dv=None, dslopes=None):
+def _call(name, q, k, v, out, lse, low, slopes, masks, options, dout=None, dq=None, dk=None, dv=None, dslopes=None):
     prefix, documents, lengths = masks
     causal, prefix_all, softcap, scale = options
     device = q.device
     batch, heads, queries, dim = q.shape
     kv_heads, keys, value_dim = v.shape[1:]
     args = _PACKED.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _address(lse), _address(slopes), _address(prefix),
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _address(lse), _address(low), _address(slopes), _address(prefix),
         _address(documents), _address(lengths), _address(dout), _address(dq), _address(dk), _address(dv),
         _address(dslopes), batch, heads, kv_heads, queries, keys, dim, value_dim,
         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
@@ -69,9 +69,13 @@ def _call(name, q, k, v, out, lse, slopes, masks, options, dout=None, dq=None, d
 
 def _forward(q, k, v, slopes, masks, options, keep):
     out = _empty(q, q.shape[1], q.shape[2], v.shape[3])
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if keep else None
-    _call("xfh_sequence_attention", q, k, v, out, lse, slopes, masks, options)
-    return out, lse
+    lse = low = None
+    if keep:                                             # for the backward pass: row sums, and what rounding left out
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+        if q.dtype == torch.bfloat16:
+            low = torch.empty((*q.shape[:3], v.shape[3]), dtype=torch.bfloat16, device=q.device)
+    _call("xfh_sequence_attention", q, k, v, out, lse, low, slopes, masks, options)
+    return out, lse, low
 
 
 class _SequenceAttention(torch.autograd.Function):
@@ -80,8 +84,8 @@ class _SequenceAttention(torch.autograd.Function):
         ctx.dtypes = q.dtype, k.dtype, v.dtype, None if slopes is None else slopes.dtype
         q, k, v = (_rows(t, dtype) for t in (q, k, v))
         s = None if slopes is None else slopes.to(torch.float32).contiguous()
-        out, lse = _forward(q, k, v, s, (prefix, documents, lengths), options, True)
-        ctx.save_for_backward(q, k, v, s, out, lse, prefix, documents, lengths)
+        out, lse, low = _forward(q, k, v, s, (prefix, documents, lengths), options, True)
+        ctx.save_for_backward(q, k, v, s, out, lse, low, prefix, documents, lengths)
         ctx.options = options
         return out
 
@@ -92,12 +96,12 @@ class _SequenceAttention(torch.autograd.Function):
 
 
 def _backward(ctx, dout):
-    q, k, v, slopes, out, lse, *masks = ctx.saved_tensors
+    q, k, v, slopes, out, lse, low, *masks = ctx.saved_tensors
     dout = _rows(dout, q.dtype)
     dq, dk, dv = (_empty(t, *t.shape[1:]) for t in (q, k, v))
     needs = ctx.needs_input_grad
     dslopes = torch.empty_like(slopes) if needs[3] else None
-    _call("xfh_sequence_attention_backward", q, k, v, out, lse, slopes, masks, ctx.options, dout, dq, dk, dv, dslopes)
+    _call("xfh_sequence_attention_backward", q, k, v, out, lse, low, slopes, masks, ctx.options, dout, dq, dk, dv, dslopes)
     grads = [dq, dk, dv, dslopes]
     for i, dtype in enumerate(ctx.dtypes):
         if not needs[i]:
