@@ -458,7 +458,8 @@ int xfh_layer_norm_backward(const void *dy, int dy_dtype, int64_t lddy, const vo
 typedef struct XfhSequenceAttention {
   const void *q, *k, *v;           /* [batch][heads][queries][dim], [batch][kv_heads][keys][dim], [..][keys][value_dim] */
   void *out;                       /* [batch][heads][queries][value_dim]; read by the backward pass */
-  float *lse;                      /* fp32 [batch][heads][queries], for the backward pass; NULL: none */
+  float *lse;                      /* statistics of the rows for the backward pass, or NULL: fp32
+                                    * [batch][heads][queries], two of these with dtype XFH_F32 */
   void *out_low;                   /* bf16 [batch][heads][queries][value_dim], contiguous, or NULL: what out's
                                     * rounding left out, which makes the backward pass more exact (bf16 only) */
   const float *slopes;             /* fp32 [heads], or NULL */

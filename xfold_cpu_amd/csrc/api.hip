@@ -973,14 +973,14 @@ static int sequence_args(const XfhSequenceAttention *p, SequenceArgs &a) {
   return XFH_OK;
 }
 
-struct SequencePlan { void *ranges, *parts; int splits; float *delta, *slope_part; };
+struct SequencePlan { void *ranges, *parts; float *delta, *slope_part; };
 static int64_t sequence_carve(Carver &cv, SequencePlan &p, const SequenceArgs &a, int dtype, bool backward, bool slopes) {
   std::memset(&p, 0, sizeof(p));
-  p.splits = !backward && dtype == XFH_BF16 ? sequence_splits(a.B, a.H, a.Hk, a.Nq, a.Nk) : 1;
-  if (p.splits > 1) p.parts = cv.take(sequence_parts_bytes(a.B, a.H, a.Nq, a.Dv, p.splits));
+  const SequenceSplits splits = sequence_splits(a, dtype);
+  const int64_t parts = backward ? sequence_backward_parts(a, splits) : sequence_forward_parts(a, splits);
+  if (parts > 0) p.parts = cv.take(parts);
   if (a.documents) p.ranges = cv.take(sequence_ranges_bytes(a.B, a.Nk));
   if (backward) {
-    if (dtype == XFH_BF16) p.parts = cv.take(sequence_bf16_backward_parts(a.B, a.H, a.Hk, a.Nq, a.Nk, a.D, a.Dv));
     p.delta = static_cast<float *>(cv.take(int64_t(a.B) * a.H * a.Nq * 4));
     if (slopes) p.slope_part = static_cast<float *>(cv.take(sequence_slope_part(a.B, a.H, a.Nq) * 4));
   }
@@ -1008,7 +1008,7 @@ int xfh_sequence_attention(const XfhSequenceAttention *args, void *workspace, in
   if (sequence_carve(cv, p, a, args->dtype, false, false) > (workspace ? workspace_bytes : 0))
     return fail(XFH_EWORKSPACE, "sequence_attention: workspace too small (need " + std::to_string(cv.used) + " bytes)");
   a.ranges = p.ranges;
-  return sequence_forward(a, args->dtype, p.parts, p.splits, as_stream(stream));
+  return sequence_forward(a, args->dtype, p.parts, as_stream(stream));
 }
 
 int64_t xfh_sequence_attention_backward_workspace_size(const XfhSequenceAttention *args) {

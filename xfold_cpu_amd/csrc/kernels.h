@@ -304,7 +304,9 @@ struct SequenceArgs {
   const void *q, *k, *v, *dout;
   void *out, *dq, *dk, *dv;
   void *low;                 // [B][H][Nq][Dv] in bf16, out before its rounding less out, or null
-  float *lse;                // [B][H][Nq], log2 of the sum of exp2 of the scores; +inf: no visible key
+  // [B][H][Nq]: bf16, log2 of the sum of exp2 of the scores (+inf: no visible key); fp32, their maximum, and a second
+  // plane with 1 / the sum (0: no visible key).
+  float *lse;
   float *delta;              // [B][H][Nq], dout . out
   float *slope_part;         // [H][B][Nq], or null
   const float *slopes;       // [H], or null
@@ -316,18 +318,28 @@ struct SequenceArgs {
   float scale, cap;
   int causal, prefix_all;
 };
+// Parts that a pass is split in where it has few work items: of the keys in the forward pass, and for dk and
+// dv of the heads that share a key and of their queries. The parts are joined in their order.
+struct Splits { int heads, tiles; };
+struct SequenceSplits { int keys; Splits queries; };
+// Parts of a forward pass: (running maximum, sum) and o [splits][B Hk][columns][Dv], columns query by query over
+// the heads of a key head.
+struct Parts {
+  float2 *ml;
+  float *o;
+  int splits;
+};
+SequenceSplits sequence_splits(const SequenceArgs &a, int dtype);
+int64_t sequence_forward_parts(const SequenceArgs &a, const SequenceSplits &n);     // bytes
+int64_t sequence_backward_parts(const SequenceArgs &a, const SequenceSplits &n);
 int64_t sequence_ranges_bytes(int64_t B, int64_t Nk);
-int sequence_ranges(const SequenceArgs &a, hipStream_t s);
-// bf16 (sequence_bf16_forward.hip, sequence_bf16_backward.hip): the keys of a forward pass with few workgroups are split, their parts joined.
-int sequence_splits(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk);
-int64_t sequence_parts_bytes(int64_t B, int64_t H, int64_t Nq, int64_t Dv, int splits);
+int64_t sequence_slope_part(int64_t B, int64_t H, int64_t Nq);   // floats
+// bf16 layouts that fit sequence_bf16_forward.hip and sequence_bf16_backward.hip, whose parts sequence.hip joins.
 bool sequence_bf16_forward_fits(const SequenceArgs &a);
 bool sequence_bf16_backward_fits(const SequenceArgs &a);
-int sequence_bf16_forward(const SequenceArgs &a, void *parts, int splits, hipStream_t s);
-int64_t sequence_bf16_backward_parts(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk, int64_t D, int64_t Dv);
-int sequence_bf16_backward(const SequenceArgs &a, void *parts, hipStream_t s);
-int sequence_forward(const SequenceArgs &a, int dtype, void *parts, int splits, hipStream_t s);
-int64_t sequence_slope_part(int64_t B, int64_t H, int64_t Nq);   // floats
+int sequence_bf16_forward(const SequenceArgs &a, const Parts &parts, hipStream_t s);
+int sequence_bf16_backward(const SequenceArgs &a, const Splits &splits, float *parts, hipStream_t s);
+int sequence_forward(const SequenceArgs &a, int dtype, void *parts, hipStream_t s);
 int sequence_backward(const SequenceArgs &a, int dtype, void *parts, float *dslopes, hipStream_t s);
 
 }  // namespace xfh

@@ -82,6 +82,28 @@ __device__ __forceinline__ float slope_gradient(float all, float far, float erro
 
 template <typename T> __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
+constexpr float kLowest = -3.402823466e38f;              // running maximum before the first key
+
+// A work item of dk and dv: 64 keys, and of the heads of their group and the tiles of their queries the share
+// [head0, head1) x [tile0, tile1) that this split has. The first keys, which causal queries see most, first.
+struct Share { int head0, head1, tile0, tile1; };
+struct KeyItem {
+  int b, hk, block, split;
+  Share share;
+  __device__ __forceinline__ KeyItem(const SequenceArgs &a, const Splits &splits) {
+    const int group = a.H / a.Hk, qtiles = (a.Nq + kTile - 1) / kTile, count = splits.heads * splits.tiles;
+    hk = blockIdx.x % a.Hk;
+    int rest = blockIdx.x / a.Hk;
+    b = rest % a.B;
+    rest /= a.B;
+    split = rest % count;
+    block = rest / count;
+    const int sh = split % splits.heads, st = split / splits.heads;
+    share = {sh * group / splits.heads, (sh + 1) * group / splits.heads, int(int64_t(st) * qtiles / splits.tiles),
+             int(int64_t(st + 1) * qtiles / splits.tiles)};
+  }
+};
+
 // A tile of a walk: its number (-1: none is left), whether this wavefront's columns see any and all of it.
 struct Step { int tile; bool mine, whole; };
 

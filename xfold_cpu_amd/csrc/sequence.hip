@@ -195,11 +195,16 @@ __device__ __forceinline__ float column_sum(float x) {
   return x + __shfl_xor(x, 32, 64);
 }
 
-// Score of a pair in log 2 units, and d(score)/d(dot) up to `scale`.
+// Score of a pair, and d(score)/d(dot) up to `scale`. bf16: in log 2 units. fp32: as it is, and its difference to
+// the row's maximum is taken before the change of base (a score of 10 changed first is off by 1e-6).
+template <typename T> __device__ __forceinline__ constexpr float score_unit() { return sizeof(T) == 4 ? 1.0f : kLog2e; }
+template <typename T> __device__ __forceinline__ float weight_of(float x, float m) {
+  return __builtin_amdgcn_exp2f(sizeof(T) == 4 ? (x - m) * kLog2e : x - m);
+}
 template <typename T> struct Scorer {
-  float scale, cap, inv_cap, slope;                    // slope in log 2 units
+  float scale, cap, inv_cap, slope;
   __device__ __forceinline__ Scorer(const SequenceArgs &a, int h)
-      : scale(a.scale), cap(a.cap), inv_cap(a.cap > 0.f ? 1.0f / a.cap : 0.f), slope(a.slopes ? a.slopes[h] * kLog2e : 0.f) {}
+      : scale(a.scale), cap(a.cap), inv_cap(a.cap > 0.f ? 1.0f / a.cap : 0.f), slope(a.slopes ? a.slopes[h] * score_unit<T>() : 0.f) {}
   __device__ __forceinline__ float operator()(const SequenceArgs &a, float dot, int pos, int key, float &factor) const {
     float x = dot * scale;
     factor = 1.f;
@@ -208,38 +213,81 @@ template <typename T> struct Scorer {
       factor = 1.f - t * t;
       x = cap * t;
     }
-    x *= kLog2e;
+    x *= score_unit<T>();
     if (a.slopes) x -= slope * fabsf(float(pos - key));
     return x;
   }
 };
 
-struct Owner { int block, h, b; };
-// Query blocks from the last to the first (a causal mask gives the last the most work), heads fastest.
-__device__ __forceinline__ Owner owner_of(int blocks, int heads, int item) {
-  const int h = item % heads, rest = item / heads;
-  return {blocks - 1 - rest % blocks, h, rest / blocks};
+// A row's statistics for the backward pass. bf16: a = its log 2 sum, P = exp2(score - a). fp32: a = its maximum, b =
+// 1 / sum, P = exp(score - a) b, in two planes of a.lse. No visible key: P is 0.
+struct Stat { float a, b; };
+template <typename T> __device__ __forceinline__ void put_stat(const SequenceArgs &a, int64_t at, float m, float l) {
+  if (sizeof(T) == 4) {
+    a.lse[at] = l == 0.f ? 0.f : m;
+    a.lse[int64_t(a.B) * a.H * a.Nq + at] = l == 0.f ? 0.f : 1.0f / l;
+  } else {
+    a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
+  }
+}
+template <typename T> __device__ __forceinline__ Stat get_stat(const SequenceArgs &a, int64_t at, bool valid) {
+  if (!valid) return {INFINITY, 0.f};
+  return {a.lse[at], sizeof(T) == 4 ? a.lse[int64_t(a.B) * a.H * a.Nq + at] : 1.f};
+}
+template <typename T> __device__ __forceinline__ float probability(float x, const Stat &s) {
+  return sizeof(T) == 4 ? weight_of<T>(x, s.a) * s.b : weight_of<T>(x, s.a);
 }
 
-template <typename T, int DP> __global__ __launch_bounds__(256) void forward_kernel(SequenceArgs a, int blocks, bool vec) {
+// What a workgroup with 64 columns of queries works on: columns and work items are as in the bf16 kernels
+// (sequence_bf16_forward.hip), query by query over the heads that share a key head.
+struct Columns {
+  int b, h, hk, i, split, c;
+  bool valid;
+  Place place;
+  Row row;
+  Span span;
+  __device__ __forceinline__ Columns(const SequenceArgs &a, int blocks, int splits) {
+    const int group = a.H / a.Hk, columns = group * a.Nq;
+    hk = blockIdx.x % a.Hk;
+    int rest = blockIdx.x / a.Hk;
+    split = rest % splits;
+    rest /= splits;
+    const int blk = blocks - 1 - rest % blocks;
+    b = rest / blocks;
+    const int c0 = blk * kTile, c1 = min(c0 + kTile, columns) - 1;
+    c = c0 + (threadIdx.x >> 6) * 16 + (threadIdx.x & 15);
+    valid = c < columns;
+    i = valid ? c / group : a.Nq;
+    h = hk * group + (valid ? c % group : 0);
+    place = place_of(a, b);
+    row = row_of(a, place, b, i);
+    span = span_of(a, place, b, c0 / group, c1 / group);
+  }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void forward_kernel(SequenceArgs a, int blocks, Parts parts, bool vec) {
   constexpr int P = DP + pitch_pad<T>();
   __shared__ __attribute__((aligned(16))) T ks[kTile * P], vs[kTile * P];
   __shared__ int ids[kTile];
-  const Owner own = owner_of(blocks, a.H, blockIdx.x);
-  const int b = own.b, h = own.h, hk = h / (a.H / a.Hk);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
-  const Place place = place_of(a, b);
-  const int i0 = own.block * kTile, i1 = min(i0 + kTile, a.Nq) - 1, i = i0 + wave * 16 + col;
-  const bool valid = i < a.Nq;
-  const Row row = row_of(a, place, b, i);
+  const Columns own(a, blocks, parts.splits);
+  const int b = own.b, h = own.h, hk = own.hk, i = own.i;
+  const int tid = threadIdx.x, lane = tid & 63, grp = lane >> 4;
+  const Place &place = own.place;
+  const bool valid = own.valid;
+  const Row &row = own.row;
   const T *kp = static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[1];
   const T *vp = static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[1];
   typename Frag<T>::type qf[DP / 32];
   load_own<T, DP>(qf, static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1] + i * a.qs[2], a.D, valid, grp, vec);
-  const Span span = span_of(a, place, b, i0, i1);
-  const int high = span.high;
-  const auto test = [&](int tile) { return key_tile_needs(a, b, tile, span, span); };
+  const auto test = [&](int tile) { return key_tile_needs(a, b, tile, own.span, own.span); };
   const Scorer<T> score(a, h);
+  int end = (own.span.high + kTile - 1) / kTile, begin = 0;
+  if (parts.splits > 1) {
+    const int per = (end + parts.splits - 1) / parts.splits;
+    begin = min(own.split * per, end);
+    end = min(begin + per, end);
+  }
 
   f32x4 o[DP / 16];
   float m, l;
@@ -248,7 +296,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void forward_ker
     l = 0.f;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Walk walk(0, (high + kTile - 1) / kTile);
+    Walk walk(begin, end);
     Step now = walk.next(test);
     TileLoad<T, DP> kt, vt;
     int id = -1;
@@ -289,7 +337,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void forward_ker
             }
           }
         const float m_new = fmaxf(m, column_max(top)), base = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = exp2_of<T>(m - base);
+        const float alpha = weight_of<T>(m, base);
         m = m_new;
         l *= alpha;
 #pragma unroll
@@ -298,7 +346,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void forward_ker
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            w[kt][e] = (seen >> (4 * kt + e)) & 1 ? exp2_of<T>(w[kt][e] - base) : 0.f;
+            w[kt][e] = (seen >> (4 * kt + e)) & 1 ? weight_of<T>(w[kt][e], base) : 0.f;
             l += w[kt][e];
           }
         add_transposed<T, DP>(vs, w, seen, strict != 0, true, o);
@@ -313,6 +361,18 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void forward_ker
   }
   l = column_sum(l);
   if (!valid) return;
+  if (parts.splits > 1) {
+    const int64_t at = (int64_t(own.split) * a.B * a.Hk + int64_t(b) * a.Hk + hk) * (a.H / a.Hk * a.Nq) + own.c;
+    if (grp == 0) parts.ml[at] = make_float2(m, l);
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = t * 16 + grp * 4 + e;
+        if (d < a.Dv) parts.o[at * a.Dv + d] = o[t][e];
+      }
+    return;
+  }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   T *op = static_cast<T *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2];
 #pragma unroll
@@ -327,7 +387,50 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void forward_ker
         if (a.low) static_cast<bf16 *>(a.low)[((int64_t(b) * a.H + h) * a.Nq + i) * a.Dv + d] = bf16(x - to_f32(r));
       }
     }
-  if (a.lse && grp == 0) a.lse[(int64_t(b) * a.H + h) * a.Nq + i] = l == 0.f ? INFINITY : m + log2f(l);
+  if (a.lse && grp == 0) put_stat<T>(a, (int64_t(b) * a.H + h) * a.Nq + i, m, l);
+}
+
+// Joins the parts of split keys, in their order: a thread per element, or per 4 where Dv is a multiple of 4.
+template <typename T, int N> __global__ __launch_bounds__(256) void join_kernel(SequenceArgs a, Parts parts) {
+  const int group = a.H / a.Hk, columns = group * a.Nq, pieces = a.Dv / N;
+  const int64_t total = int64_t(a.B) * a.Hk * columns, at = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= total * pieces) return;
+  const int64_t column = at / pieces;
+  const int d = int(at - column * pieces) * N;
+  float top = kLowest;
+  for (int s = 0; s < parts.splits; ++s) top = fmaxf(top, parts.ml[s * total + column].x);
+  float sum = 0.f, v[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = 0.f;
+  for (int s = 0; s < parts.splits; ++s) {
+    const float2 p = parts.ml[s * total + column];
+    const float f = weight_of<T>(p.x, top);
+    float o[N];
+    __builtin_memcpy(o, __builtin_assume_aligned(parts.o + (s * total + column) * a.Dv + d, 4 * N), 4 * N);
+    sum += f * p.y;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] += f * o[e];
+  }
+  const int c = int(column % columns), bk = int(column / columns), hk = bk % a.Hk, b = bk / a.Hk;
+  const int i = c / group, h = hk * group + c % group;
+  const int64_t row = (int64_t(b) * a.H + h) * a.Nq + i;
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  T r[N];
+  bf16 low[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float x = v[e] * inv;
+    r[e] = from_f32<T>(x);
+    low[e] = bf16(x - to_f32(r[e]));
+  }
+  T *out = static_cast<T *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2] + d;
+#pragma unroll
+  for (int e = 0; e < N; ++e) out[e] = r[e];
+  if (a.low) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) static_cast<bf16 *>(a.low)[row * a.Dv + d + e] = low[e];
+  }
+  if (a.lse && d == 0) put_stat<T>(a, row, top, sum);
 }
 
 // dq of 64 queries, their delta = dout . out (for dk and dv), and the slopes' part of each query,
@@ -338,13 +441,12 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
   constexpr int P = DP + pitch_pad<T>();
   __shared__ __attribute__((aligned(16))) T ks[kTile * P], vs[kTile * P];
   __shared__ int ids[kTile];
-  const Owner own = owner_of(blocks, a.H, blockIdx.x);
-  const int b = own.b, h = own.h, hk = h / (a.H / a.Hk);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
-  const Place place = place_of(a, b);
-  const int i0 = own.block * kTile, i1 = min(i0 + kTile, a.Nq) - 1, i = i0 + wave * 16 + col;
-  const bool valid = i < a.Nq;
-  const Row row = row_of(a, place, b, i);
+  const Columns own(a, blocks, 1);
+  const int b = own.b, h = own.h, hk = own.hk, i = own.i;
+  const int tid = threadIdx.x, lane = tid & 63, grp = lane >> 4;
+  const Place &place = own.place;
+  const bool valid = own.valid;
+  const Row &row = own.row;
   const T *kp = static_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[1];
   const T *vp = static_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[1];
   typename Frag<T>::type qf[DP / 32], gf[DP / 32];
@@ -359,11 +461,9 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
     for (int d0 = grp * 8; d0 < a.Dv; d0 += 32)
       for (int d = d0; d < min(d0 + 8, a.Dv); ++d) delta += to_f32(gp[d]) * (to_f32(op[d]) + (low ? to_f32(low[d]) : 0.f));
   delta = column_sum(delta);
-  const float lse = valid ? a.lse[at] : INFINITY;
+  const Stat stat = get_stat<T>(a, at, valid);
   if (valid && grp == 0) a.delta[at] = delta;
-  const Span span = span_of(a, place, b, i0, i1);
-  const int high = span.high;
-  const auto test = [&](int tile) { return key_tile_needs(a, b, tile, span, span); };
+  const auto test = [&](int tile) { return key_tile_needs(a, b, tile, own.span, own.span); };
   const Scorer<T> score(a, h);
 
   f32x4 dq[DP / 16];
@@ -372,7 +472,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
     all = far = error = far_error = 0.f;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) dq[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Walk walk(0, (high + kTile - 1) / kTile);
+    Walk walk(0, (own.span.high + kTile - 1) / kTile);
     Step now = walk.next(test);
     TileLoad<T, DP> kt, vt;
     int id = -1;
@@ -406,7 +506,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
             const bool see = valid && (whole || (key < row.limit && (!a.documents || ids[r] == row.document)));
             float factor;
             const float x = score(a, s[kt][e], row.pos, key, factor);
-            const float p = see ? exp2_of<T>(x - lse) : 0.f;
+            const float p = see ? probability<T>(x, stat) : 0.f;
             const float ds = see ? p * (dp[kt][e] - delta) : 0.f;
             w[kt][e] = ds * factor;
             seen |= see ? 1u << (4 * kt + e) : 0u;
@@ -447,14 +547,16 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
   }
 }
 
-// dk and dv of 64 keys: over the heads that share them and the queries that see them.
-template <typename T, int DP> __global__ __launch_bounds__(256) void dkv_kernel(SequenceArgs a, int blocks, bool vec) {
+// dk and dv of 64 keys: over the heads that share them and the queries that see them (of a work item's share).
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void dkv_kernel(SequenceArgs a, Splits splits, float *parts, bool vec) {
   constexpr int P = DP + pitch_pad<T>();
   __shared__ __attribute__((aligned(16))) T qs[kTile * P], gs[kTile * P];
   __shared__ Row rows[kTile];
-  __shared__ float lses[kTile], deltas[kTile];
-  const int hk = blockIdx.x % a.Hk, rest = blockIdx.x / a.Hk, group = a.H / a.Hk;
-  const int block = rest % blocks, b = rest / blocks;      // the first keys, which causal queries see most, first
+  __shared__ Stat stats[kTile];
+  __shared__ float deltas[kTile];
+  const KeyItem item(a, splits);
+  const int hk = item.hk, b = item.b, block = item.block, group = a.H / a.Hk;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
   const Place place = place_of(a, b);
   const int k0 = block * kTile, key = k0 + wave * 16 + col;
@@ -468,13 +570,12 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dkv_kernel(
     id = valid ? a.documents[int64_t(b) * a.documents_stride + key] : -1;
     mine = static_cast<const Range *>(a.ranges)[int64_t(b) * a.tiles + block];
   }
-  const int qtiles = (a.Nq + kTile - 1) / kTile;
 
   f32x4 dk[DP / 16], dv[DP / 16];
   for (int strict = 0; strict < 2; ++strict) {
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) dk[t] = dv[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int g = 0; g < group; ++g) {
+    for (int g = item.share.head0; g < item.share.head1; ++g) {
       const int h = hk * group + g;
       const T *qp = static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1];
       const T *gp = static_cast<const T *>(a.dout) + b * a.gs[0] + h * a.gs[1];
@@ -490,18 +591,19 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dkv_kernel(
         }
         return n;
       };
-      Walk walk(0, qtiles);
+      Walk walk(item.share.tile0, item.share.tile1);
       Step now = walk.next(test);
       TileLoad<T, DP> qt, gt;
       Row next_row{};
-      float next_lse = INFINITY, next_delta = 0.f;
+      Stat next_stat{INFINITY, 0.f};
+      float next_delta = 0.f;
       const auto fetch = [&](int i0) {
         qt.fetch(qp, a.qs[2], i0, a.Nq, a.D, vec);
         gt.fetch(gp, a.gs[2], i0, a.Nq, a.Dv, vec);
         if (tid < kTile) {
           const int i = i0 + tid;
           next_row = row_of(a, place, b, i);
-          next_lse = i < a.Nq ? a.lse[at + i] : INFINITY;
+          next_stat = get_stat<T>(a, at + i, i < a.Nq);
           next_delta = i < a.Nq ? a.delta[at + i] : 0.f;
         }
       };
@@ -515,7 +617,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dkv_kernel(
           gt.put(gs, gp, a.gs[2], i0, a.Nq, a.Dv, vec);
           if (tid < kTile) {
             rows[tid] = next_row;
-            lses[tid] = next_lse;
+            stats[tid] = next_stat;
             deltas[tid] = next_delta;
           }
           __syncthreads();
@@ -535,7 +637,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dkv_kernel(
               const bool see = valid && (all || (key < row.limit && (!a.documents || id == row.document)));
               float factor;
               const float x = score(a, s[kt][e], row.pos, key, factor);
-              pw[kt][e] = see ? exp2_of<T>(x - lses[r]) : 0.f;
+              pw[kt][e] = see ? probability<T>(x, stats[r]) : 0.f;
               w[kt][e] = see ? pw[kt][e] * (dp[kt][e] - deltas[r]) * factor : 0.f;
               seen |= see ? 1u << (4 * kt + e) : 0u;
             }
@@ -552,6 +654,18 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dkv_kernel(
     if (!__syncthreads_or(valid && bad)) break;
   }
   if (key >= a.Nk) return;                                 // (keys beyond a length: zeros)
+  if (splits.heads * splits.tiles > 1) {
+    float *to = parts + ((int64_t(item.split) * a.B * a.Hk + int64_t(b) * a.Hk + hk) * a.Nk + key) * (a.D + a.Dv);
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = t * 16 + grp * 4 + e;
+        if (d < a.D) to[d] = valid ? dk[t][e] : 0.f;
+        if (d < a.Dv) to[a.D + d] = valid ? dv[t][e] : 0.f;
+      }
+    return;
+  }
   T *kout = static_cast<T *>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2];
   T *vout = static_cast<T *>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2];
 #pragma unroll
@@ -562,6 +676,30 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dkv_kernel(
       if (d < a.D) kout[d] = from_f32<T>(valid ? dk[t][e] * a.scale : 0.f);
       if (d < a.Dv) vout[d] = from_f32<T>(valid ? dv[t][e] : 0.f);
     }
+}
+
+// dk and dv from the parts of their work items, in order: a thread per element, or per 4.
+template <typename T, int N> __global__ __launch_bounds__(256) void dkv_join_kernel(SequenceArgs a, int splits, const float *parts) {
+  const int width = a.D + a.Dv, pieces = width / N;
+  const int64_t rows = int64_t(a.B) * a.Hk * a.Nk, at = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= rows * pieces) return;
+  const int64_t row = at / pieces;
+  const int d = int(at - row * pieces) * N;
+  float sum[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) sum[e] = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    float p[N];
+    __builtin_memcpy(p, __builtin_assume_aligned(parts + (s * rows + row) * width + d, 4 * N), 4 * N);
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum[e] += p[e];
+  }
+  const int key = int(row % a.Nk), bk = int(row / a.Nk), hk = bk % a.Hk, b = bk / a.Hk;
+  T *out = d < a.D ? static_cast<T *>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2] + d
+                   : static_cast<T *>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2] + d - a.D;
+  const float scale = d < a.D ? a.scale : 1.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) out[e] = from_f32<T>(sum[e] * scale);
 }
 
 // dslopes[h]: the sum of its parts, in their order.
@@ -587,25 +725,27 @@ template <typename T> bool vector_rows(std::initializer_list<std::pair<const voi
   return true;
 }
 
-template <typename T, int DP> int launch_forward(const SequenceArgs &a, hipStream_t s) {
-  const int64_t blocks = ceil_div(a.Nq, int64_t(kTile));
+template <typename T, int DP> int launch_forward(const SequenceArgs &a, const Parts &parts, hipStream_t s) {
+  const int64_t blocks = ceil_div(int64_t(a.H / a.Hk) * a.Nq, int64_t(kTile));
   const bool vec = vector_rows<T>({{a.q, a.qs}, {a.k, a.ks}}, a.D) && vector_rows<T>({{a.v, a.vs}}, a.Dv);
-  forward_kernel<T, DP><<<dim3(unsigned(blocks * a.H * a.B)), 256, 0, s>>>(a, int(blocks), vec);
+  forward_kernel<T, DP><<<dim3(unsigned(blocks * a.Hk * a.B * parts.splits)), 256, 0, s>>>(a, int(blocks), parts, vec);
   return check_launch("sequence_attention");
 }
 
-template <typename T, int DP> int launch_backward(const SequenceArgs &a, hipStream_t s) {
-  const int64_t qblocks = ceil_div(a.Nq, int64_t(kTile)), kblocks = ceil_div(a.Nk, int64_t(kTile));
+template <typename T, int DP> int launch_backward(const SequenceArgs &a, const Splits &splits, float *parts, hipStream_t s) {
+  const int64_t qblocks = ceil_div(int64_t(a.H / a.Hk) * a.Nq, int64_t(kTile)), kblocks = ceil_div(a.Nk, int64_t(kTile));
   const bool vec = vector_rows<T>({{a.k, a.ks}, {a.q, a.qs}}, a.D) && vector_rows<T>({{a.v, a.vs}, {a.dout, a.gs}}, a.Dv);
-  if (qblocks > 0 && a.H > 0) dq_kernel<T, DP><<<dim3(unsigned(qblocks * a.H * a.B)), 256, 0, s>>>(a, int(qblocks), vec);
+  if (qblocks > 0) dq_kernel<T, DP><<<dim3(unsigned(qblocks * a.Hk * a.B)), 256, 0, s>>>(a, int(qblocks), vec);
   XFH_TRY(check_launch("sequence_attention_backward"));
-  if (kblocks > 0) dkv_kernel<T, DP><<<dim3(unsigned(kblocks * a.Hk * a.B)), 256, 0, s>>>(a, int(kblocks), vec);
+  if (kblocks > 0)
+    dkv_kernel<T, DP><<<dim3(unsigned(kblocks * a.Hk * a.B * splits.heads * splits.tiles)), 256, 0, s>>>(a, splits, parts, vec);
   return check_launch("sequence_attention_backward");
 }
 
 int check_grid(const SequenceArgs &a) {
-  const int64_t most = std::max(ceil_div(int64_t(a.Nq), int64_t(kTile)) * a.H, ceil_div(int64_t(a.Nk), int64_t(kTile)) * a.Hk) * a.B;
-  if (most > (int64_t(1) << 31) - 1) return fail(XFH_EUNSUPPORTED, "sequence_attention: problem too large");
+  // At most 64 splits of a work item's keys, and those only of few work items.
+  const int64_t most = std::max((ceil_div(int64_t(a.Nq), int64_t(kTile)) + 1) * a.H, ceil_div(int64_t(a.Nk), int64_t(kTile)) * a.Hk) * a.B;
+  if (most > (int64_t(1) << 31) - 65536 || int64_t(a.H / std::max(a.Hk, 1)) * a.Nq > (int64_t(1) << 31) - 256) return fail(XFH_EUNSUPPORTED, "sequence_attention: problem too large");
   return XFH_OK;
 }
 
@@ -621,36 +761,101 @@ int sequence_ranges(const SequenceArgs &a, hipStream_t s) {
   return check_launch("sequence_attention");
 }
 
-int sequence_forward(const SequenceArgs &a, int dtype, void *parts, int splits, hipStream_t s) {
+SequenceSplits sequence_splits(const SequenceArgs &a, int dtype) {
+  SequenceSplits n{1, {1, 1}};
+  if (a.B == 0 || a.H == 0 || a.Hk == 0) return n;
+  const bool bf = dtype == XFH_BF16 && sequence_bf16_forward_fits(a);
+  const int64_t columns = int64_t(a.H / a.Hk) * a.Nq, single = int64_t(a.B) * a.Hk;
+  if (columns > 0 && a.Nk > 0) {
+    // Keys are split until there are about 512 work items (two workgroups per CU), down to 8 tiles each, 4 of
+    // single tokens. 4 x 200 queries of 5000 keys in bf16: 77 + 9 us in two splits (224 work items unsplit), 115 in one.
+    const int64_t items = columns <= 32 ? single : single * ceil_div(columns, int64_t(bf ? 128 : kTile));
+    const int64_t most = ceil_div(int64_t(a.Nk), int64_t(columns <= 32 ? 256 : 512));
+    n.keys = int(std::max(int64_t(1), std::min(std::min(most, 512 / items), int64_t(64))));
+  }
+  if (a.Nk > 0 && a.Nq > 0) {
+    // dk and dv are summed in parts (heads first, then runs of queries of at least 4 tiles) until there are about 1024
+    // work items, so that long and short ones even out. Packed training 2 x 4096: 175 + 16 us in two parts, 275 in one.
+    const int64_t items = ceil_div(int64_t(a.Nk), int64_t(kTile)) * single, want = std::max(int64_t(1), 1024 / items);
+    const int64_t heads = std::min(int64_t(a.H / a.Hk), want);
+    const int64_t tiles = std::min(want / heads, ceil_div(int64_t(a.Nq), int64_t(4 * kTile)));
+    n.queries = {int(heads), int(std::max(int64_t(1), std::min(tiles, int64_t(16))))};
+  }
+  return n;
+}
+int64_t sequence_forward_parts(const SequenceArgs &a, const SequenceSplits &n) {
+  const int64_t rows = n.keys * int64_t(a.B) * a.H * a.Nq;
+  return n.keys <= 1 ? 0 : align_up(rows, 2) * 8 + rows * a.Dv * 4;
+}
+int64_t sequence_backward_parts(const SequenceArgs &a, const SequenceSplits &n) {
+  const int64_t count = int64_t(n.queries.heads) * n.queries.tiles;
+  return count <= 1 ? 0 : count * a.B * a.Hk * a.Nk * (a.D + a.Dv) * 4;
+}
+
+int sequence_forward(const SequenceArgs &a, int dtype, void *memory, hipStream_t s) {
   if (a.B == 0 || a.H == 0 || a.Nq == 0) return XFH_OK;
   XFH_TRY(check_grid(a));
   XFH_TRY(sequence_ranges(a, s));
-  if (dtype == XFH_BF16 && sequence_bf16_forward_fits(a)) return sequence_bf16_forward(a, parts, splits, s);
-  const int d = std::max(a.D, a.Dv);
-#define XFH_SEQ_FORWARD(DP) return dtype == XFH_BF16 ? launch_forward<bf16, DP>(a, s) : launch_forward<float, DP>(a, s)
-  if (d <= 32) XFH_SEQ_FORWARD(32);
-  if (d <= 64) XFH_SEQ_FORWARD(64);
-  if (d <= 96) XFH_SEQ_FORWARD(96);
-  XFH_SEQ_FORWARD(128);
+  const int splits = sequence_splits(a, dtype).keys;
+  Parts parts{static_cast<float2 *>(memory), nullptr, splits};
+  if (splits > 1) parts.o = reinterpret_cast<float *>(parts.ml + align_up(splits * int64_t(a.B) * a.H * a.Nq, 2));   // (on 16 bytes)
+  if (dtype == XFH_BF16 && sequence_bf16_forward_fits(a)) {
+    XFH_TRY(sequence_bf16_forward(a, parts, s));
+  } else {
+    const int d = std::max(a.D, a.Dv);
+    int status = XFH_OK;
+#define XFH_SEQ_FORWARD(DP) status = dtype == XFH_BF16 ? launch_forward<bf16, DP>(a, parts, s) : launch_forward<float, DP>(a, parts, s)
+    if (d <= 32) XFH_SEQ_FORWARD(32);
+    else if (d <= 64) XFH_SEQ_FORWARD(64);
+    else if (d <= 96) XFH_SEQ_FORWARD(96);
+    else XFH_SEQ_FORWARD(128);
 #undef XFH_SEQ_FORWARD
+    if (status != XFH_OK) return status;
+  }
+  if (splits <= 1) return XFH_OK;
+  const bool quads = a.Dv % 4 == 0;
+  const dim3 grid(unsigned(ceil_div(int64_t(a.B) * a.H * a.Nq * (quads ? a.Dv / 4 : a.Dv), int64_t(256))));
+  if (dtype == XFH_BF16) {
+    if (quads) join_kernel<bf16, 4><<<grid, 256, 0, s>>>(a, parts);
+    else join_kernel<bf16, 1><<<grid, 256, 0, s>>>(a, parts);
+  } else {
+    if (quads) join_kernel<float, 4><<<grid, 256, 0, s>>>(a, parts);
+    else join_kernel<float, 1><<<grid, 256, 0, s>>>(a, parts);
+  }
+  return check_launch("sequence_attention");
 }
 
 int64_t sequence_slope_part(int64_t B, int64_t H, int64_t Nq) { return H * B * Nq; }
 
-int sequence_backward(const SequenceArgs &a, int dtype, void *parts, float *dslopes, hipStream_t s) {
+int sequence_backward(const SequenceArgs &a, int dtype, void *memory, float *dslopes, hipStream_t s) {
+  float *parts = static_cast<float *>(memory);
   if (a.B > 0 && a.Hk > 0) {
     XFH_TRY(check_grid(a));
     XFH_TRY(sequence_ranges(a, s));
-    const int d = std::max(a.D, a.Dv);
+    const Splits splits = sequence_splits(a, dtype).queries;
+    const int d = std::max(a.D, a.Dv), count = splits.heads * splits.tiles;
     int status = XFH_OK;
-#define XFH_SEQ_BACKWARD(DP) status = dtype == XFH_BF16 ? launch_backward<bf16, DP>(a, s) : launch_backward<float, DP>(a, s)
-    if (dtype == XFH_BF16 && sequence_bf16_backward_fits(a)) status = sequence_bf16_backward(a, parts, s);
+#define XFH_SEQ_BACKWARD(DP) \
+  status = dtype == XFH_BF16 ? launch_backward<bf16, DP>(a, splits, parts, s) : launch_backward<float, DP>(a, splits, parts, s)
+    if (dtype == XFH_BF16 && sequence_bf16_backward_fits(a)) status = sequence_bf16_backward(a, splits, parts, s);
     else if (d <= 32) XFH_SEQ_BACKWARD(32);
     else if (d <= 64) XFH_SEQ_BACKWARD(64);
     else if (d <= 96) XFH_SEQ_BACKWARD(96);
     else XFH_SEQ_BACKWARD(128);
 #undef XFH_SEQ_BACKWARD
     if (status != XFH_OK) return status;
+    if (count > 1) {
+      const bool quads = a.D % 4 == 0 && a.Dv % 4 == 0;
+      const dim3 grid(unsigned(ceil_div(int64_t(a.B) * a.Hk * a.Nk * ((a.D + a.Dv) / (quads ? 4 : 1)), int64_t(256))));
+      if (dtype == XFH_BF16) {
+        if (quads) dkv_join_kernel<bf16, 4><<<grid, 256, 0, s>>>(a, count, parts);
+        else dkv_join_kernel<bf16, 1><<<grid, 256, 0, s>>>(a, count, parts);
+      } else {
+        if (quads) dkv_join_kernel<float, 4><<<grid, 256, 0, s>>>(a, count, parts);
+        else dkv_join_kernel<float, 1><<<grid, 256, 0, s>>>(a, count, parts);
+      }
+      XFH_TRY(check_launch("sequence_attention_backward"));
+    }
   }
   if (!dslopes || a.H == 0) return XFH_OK;
   dslopes_kernel<<<dim3(unsigned(a.H)), 256, 0, s>>>(a.slope_part, int64_t(a.B) * a.Nq, dslopes);

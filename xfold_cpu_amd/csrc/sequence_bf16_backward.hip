@@ -187,14 +187,9 @@ __device__ __forceinline__ uint32_t hide_queries(const Marks &marks, int half, i
   return seen;
 }
 
-constexpr int kKeys = 64;                                // keys of a workgroup
-
 // Tiles of LDS in use: with two, the next one is on its way during a step. At DL = 128 two would leave room for
 // one workgroup per CU; two workgroups with one stage each hide each other's loads.
 template <class D> constexpr int kDkvStages = D::DL == 128 ? 1 : 2;
-// The heads and tiles of queries of a work item, [head0, head1) and [tile0, tile1).
-struct Share { int head0, head1, tile0, tile1; };
-struct Splits { int heads, tiles; };
 
 // What the two wavefronts of a key group hand each other: P and dS of 32 queries as B fragments, and, in
 // the rare form, the bits of the pairs that are seen.
@@ -352,18 +347,13 @@ __global__ __launch_bounds__(256, 2) void dkv_bf16_kernel(SequenceArgs a, Splits
   __shared__ __attribute__((aligned(1024))) float stats0[2 * kTile], stats1[STAGES == 2 ? 2 * kTile : 4];
   __shared__ __attribute__((aligned(16))) Exchange exchange[4];
   __shared__ __attribute__((aligned(16))) Marks marks[4];
-  const int hk = blockIdx.x % a.Hk;
-  int rest = blockIdx.x / a.Hk;
-  const int b = rest % a.B;
-  rest /= a.B;
-  const int count = splits.heads * splits.tiles, split = rest % count, blk = rest / count;
+  const KeyItem item(a, splits);
+  const int hk = item.hk, b = item.b;
+  const Share &share = item.share;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave >> 1;
-  const int group = a.H / a.Hk, qtiles = (a.Nq + kTile - 1) / kTile, sh = split % splits.heads, st = split / splits.heads;
-  const Share share{sh * group / splits.heads, (sh + 1) * group / splits.heads, int(int64_t(st) * qtiles / splits.tiles),
-                    int(int64_t(st + 1) * qtiles / splits.tiles)};
   const Lane<D> ln;
   const Place place = place_of(a, b);
-  const int kb = blk * kKeys, kw = kb + (wave & 1) * 32, key = kw + ln.col;
+  const int kb = item.block * kTile, kw = kb + (wave & 1) * 32, key = kw + ln.col;
   const bool valid = key < place.n;
   bf16x8 kf[D::KS], vf[D::KS];
   own_row<D>(kf, static_cast<const bf16 *>(a.k) + b * a.ks[0] + hk * a.ks[1] + key * a.ks[2], a.D, valid, ln.half);
@@ -385,8 +375,8 @@ __global__ __launch_bounds__(256, 2) void dkv_bf16_kernel(SequenceArgs a, Splits
     }
   }
   const int d0 = part * T * 32;
-  if (count > 1) {
-    float *to = parts + ((int64_t(split) * a.B * a.Hk + int64_t(b) * a.Hk + hk) * a.Nk + key) * (a.D + a.Dv);
+  if (splits.heads * splits.tiles > 1) {
+    float *to = parts + ((int64_t(item.split) * a.B * a.Hk + int64_t(b) * a.Hk + hk) * a.Nk + key) * (a.D + a.Dv);
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
@@ -402,35 +392,6 @@ __global__ __launch_bounds__(256, 2) void dkv_bf16_kernel(SequenceArgs a, Splits
   store_column(static_cast<bf16 *>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2] + d0, a.Dv - d0, dv, 1.f, ln.half);
 }
 
-// dk and dv from the parts of their work items, in order: a thread per 4 elements.
-__global__ __launch_bounds__(256) void dkv_join_kernel(SequenceArgs a, int splits, const float *parts) {
-  const int width = a.D + a.Dv, quads = width / 4;
-  const int64_t rows = int64_t(a.B) * a.Hk * a.Nk, at = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= rows * quads) return;
-  const int64_t row = at / quads;
-  const int d = int(at - row * quads) * 4;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const f32x4 *>(parts + (s * rows + row) * width + d);
-  const int key = int(row % a.Nk), bk = int(row / a.Nk), hk = bk % a.Hk, b = bk / a.Hk;
-  bf16 *out = d < a.D ? static_cast<bf16 *>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2] + d
-                      : static_cast<bf16 *>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2] + d - a.D;
-  const float scale = d < a.D ? a.scale : 1.f;
-  bf16x4 v;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = static_cast<bf16>(sum[e] * scale);
-  *reinterpret_cast<bf16x4 *>(out) = v;
-}
-
-// Parts of the heads and of the queries that dk and dv are summed in: at least about 1024 work items (two rounds
-// of two workgroups per CU), so that long and short ones even out.
-Splits dkv_splits(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk) {
-  if (B == 0 || Hk == 0 || H == 0 || Nk == 0) return {1, 1};
-  const int64_t items = ceil_div(Nk, int64_t(kKeys)) * B * Hk, want = std::max(int64_t(1), 1024 / items);
-  const int64_t heads = std::min(H / Hk, want);
-  const int64_t tiles = std::max(int64_t(1), std::min(want / heads, ceil_div(Nq, int64_t(4 * kTile))));
-  return {int(heads), int(std::min(tiles, int64_t(16)))};
-}
-
 }  // namespace
 
 bool sequence_bf16_backward_fits(const SequenceArgs &a) {
@@ -439,27 +400,16 @@ bool sequence_bf16_backward_fits(const SequenceArgs &a) {
 }
 
 
-int64_t sequence_bf16_backward_parts(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk, int64_t D, int64_t Dv) {
-  const Splits n = dkv_splits(B, H, Hk, Nq, Nk);
-  return n.heads * n.tiles <= 1 ? 0 : int64_t(n.heads) * n.tiles * B * Hk * Nk * (D + Dv) * 4;
-}
-
-int sequence_bf16_backward(const SequenceArgs &a, void *parts, hipStream_t s) {
-  const int64_t blocks = ceil_div(int64_t(a.H / a.Hk) * a.Nq, int64_t(kColumns)), kblocks = ceil_div(int64_t(a.Nk), int64_t(kKeys));
+int sequence_bf16_backward(const SequenceArgs &a, const Splits &splits, float *parts, hipStream_t s) {
+  const int64_t blocks = ceil_div(int64_t(a.H / a.Hk) * a.Nq, int64_t(kColumns)), kblocks = ceil_div(int64_t(a.Nk), int64_t(kTile));
   return with_dims(a, [&](auto dim, auto mode) {
     typedef decltype(dim) D;
+    typedef Dim<D::DL < 64 ? 64 : D::DL, D::KS, D::DT + D::DT % 2> E;    // (two wavefronts share the head dim)
     constexpr int MODE = decltype(mode)::value;
     if (blocks > 0) dq_bf16_kernel<D, MODE><<<dim3(unsigned(blocks * a.Hk * a.B)), 256, 0, s>>>(a, int(blocks));
     XFH_TRY(check_launch("sequence_attention_backward"));
-    typedef Dim<D::DL < 64 ? 64 : D::DL, D::KS, D::DT + D::DT % 2> E;    // (two wavefronts share the head dim)
-    if (kblocks == 0) return int(XFH_OK);
-    const Splits splits = dkv_splits(a.B, a.H, a.Hk, a.Nq, a.Nk);
-    const int count = splits.heads * splits.tiles;
-    dkv_bf16_kernel<E, MODE><<<dim3(unsigned(kblocks * a.Hk * a.B * count)), 256, 0, s>>>(a, splits, static_cast<float *>(parts));
-    XFH_TRY(check_launch("sequence_attention_backward"));
-    if (count > 1)
-      dkv_join_kernel<<<dim3(unsigned(ceil_div(int64_t(a.B) * a.Hk * a.Nk * ((a.D + a.Dv) / 4), int64_t(256)))), 256, 0, s>>>(
-          a, count, static_cast<const float *>(parts));
+    if (kblocks > 0)
+      dkv_bf16_kernel<E, MODE><<<dim3(unsigned(kblocks * a.Hk * a.B * splits.heads * splits.tiles)), 256, 0, s>>>(a, splits, parts);
     return check_launch("sequence_attention_backward");
   });
 }

@@ -12,7 +12,6 @@ namespace {
 using namespace seq;
 
 constexpr float kSlack = 8.0f;                           // log 2 units that a score may exceed the maximum in use
-constexpr float kLowest = -3.402823466e38f;              // running maximum before the first key
 
 // One wavefront's 64 keys of a tile: scores, running maximum and sum, o += P V. The maximum in use is
 // raised (and o and l scaled) only when a score exceeds it by kSlack, so weights are at most 2^kSlack.
@@ -64,13 +63,6 @@ __device__ __forceinline__ void forward_tile(const SequenceArgs &a, const Lane<D
     add_product<STRICT, true>(vf, weights(w[kk / 2], 8 * (kk & 1)), weights_seen(seen[kk / 2], 8 * (kk & 1)), o);
   }
 }
-
-// Where the parts of a forward pass whose keys are split go: o [splits][B Hk][columns][Dv], (m, l) beside it.
-struct Parts {
-  float *o;
-  float2 *ml;
-  int splits;
-};
 
 // The stages are arrays of their own, which the code takes in turns: reads of one are then known not to
 // depend on the direct loads in flight to the other (else the compiler waits for these before every read).
@@ -301,40 +293,6 @@ __global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, int 
   }
 }
 
-// Joins the parts of split keys, in their order: a thread per 4 elements (Dv is a multiple of 8 here).
-__global__ __launch_bounds__(256) void join_kernel(SequenceArgs a, Parts parts) {
-  const int group = a.H / a.Hk, columns = group * a.Nq, quads = a.Dv / 4;
-  const int64_t total = int64_t(a.B) * a.Hk * columns, at = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= total * quads) return;
-  const int64_t column = at / quads;
-  const int d = int(at - column * quads) * 4;
-  float top = kLowest;
-  for (int s = 0; s < parts.splits; ++s) top = fmaxf(top, parts.ml[s * total + column].x);
-  float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < parts.splits; ++s) {
-    const float2 p = parts.ml[s * total + column];
-    const float4 o = *reinterpret_cast<const float4 *>(parts.o + (s * total + column) * a.Dv + d);
-    const float f = __builtin_amdgcn_exp2f(p.x - top);
-    sum += f * p.y;
-    v[0] += f * o.x; v[1] += f * o.y; v[2] += f * o.z; v[3] += f * o.w;
-  }
-  const int c = int(column % columns), bk = int(column / columns), hk = bk % a.Hk, b = bk / a.Hk;
-  const int i = c / group, h = hk * group + c % group;
-  bf16 *out = static_cast<bf16 *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2] + d;
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  bf16x4 r;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) r[e] = static_cast<bf16>(v[e] * inv);
-  *reinterpret_cast<bf16x4 *>(out) = r;
-  if (a.low) {
-    bf16x4 u;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = static_cast<bf16>(v[e] * inv - static_cast<float>(r[e]));
-    *reinterpret_cast<bf16x4 *>(static_cast<bf16 *>(a.low) + ((int64_t(b) * a.H + h) * a.Nq + i) * a.Dv + d) = u;
-  }
-  if (a.lse && d == 0) a.lse[(int64_t(b) * a.H + h) * a.Nq + i] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
-}
-
 }  // namespace
 
 bool sequence_bf16_forward_fits(const SequenceArgs &a) {
@@ -342,34 +300,17 @@ bool sequence_bf16_forward_fits(const SequenceArgs &a) {
          reinterpret_cast<uintptr_t>(a.low) % 8 == 0 && int64_t(a.H / a.Hk) * a.Nq < (int64_t(1) << 31) - 256;
 }
 
-int sequence_splits(int64_t B, int64_t H, int64_t Hk, int64_t Nq, int64_t Nk) {
-  if (H == 0 || Hk == 0 || B == 0) return 1;
-  const int64_t columns = H / Hk * Nq;
-  const int64_t items = columns <= 32 ? B * Hk : B * Hk * ceil_div(columns, int64_t(kColumns));
-  const int64_t most = columns <= 32 ? ceil_div(Nk, int64_t(256)) : ceil_div(Nk, int64_t(512));
-  return int(std::max(int64_t(1), std::min(std::min(most, 512 / items), int64_t(64))));
-}
-
-int64_t sequence_parts_bytes(int64_t B, int64_t H, int64_t Nq, int64_t Dv, int splits) {
-  return splits <= 1 ? 0 : splits * B * H * Nq * (Dv * 4 + 8);
-}
-
-int sequence_bf16_forward(const SequenceArgs &a, void *parts_memory, int splits, hipStream_t s) {
+int sequence_bf16_forward(const SequenceArgs &a, const Parts &parts, hipStream_t s) {
   const int64_t columns = int64_t(a.H / a.Hk) * a.Nq;
-  Parts parts{static_cast<float *>(parts_memory), nullptr, splits};
-  if (splits > 1) parts.ml = reinterpret_cast<float2 *>(parts.o + splits * int64_t(a.B) * a.H * a.Nq * a.Dv);
   const int64_t blocks = columns <= 32 ? 1 : ceil_div(columns, int64_t(kColumns));
-  const dim3 grid(unsigned(blocks * a.Hk * a.B * splits));
-  XFH_TRY(with_dims(a, [&](auto dim, auto mode) {
+  const dim3 grid(unsigned(blocks * a.Hk * a.B * parts.splits));
+  return with_dims(a, [&](auto dim, auto mode) {
     typedef decltype(dim) D;
     constexpr int MODE = decltype(mode)::value;
     if (columns <= 32) token_bf16_kernel<D, MODE><<<grid, 256, 0, s>>>(a, 1, parts);
     else forward_bf16_kernel<D, MODE><<<grid, 256, 0, s>>>(a, int(blocks), parts);
     return check_launch("sequence_attention");
-  }));
-  if (splits <= 1) return XFH_OK;
-  join_kernel<<<dim3(unsigned(ceil_div(int64_t(a.B) * a.H * a.Nq * (a.Dv / 4), int64_t(256)))), 256, 0, s>>>(a, parts);
-  return check_launch("sequence_attention");
+  });
 }
 
 }  // namespace xfh

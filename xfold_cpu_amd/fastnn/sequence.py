@@ -71,8 +71,9 @@ def _forward(q, k, v, slopes, masks, options, keep):
     out = _empty(q, q.shape[1], q.shape[2], v.shape[3])
     lse = low = None
     if keep:                                             # for the backward pass: row sums, and what rounding left out
-        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-        if q.dtype == torch.bfloat16:
+        single = q.dtype == torch.float32
+        lse = torch.empty((1 + single, *q.shape[:3]), dtype=torch.float32, device=q.device)
+        if not single:
             low = torch.empty((*q.shape[:3], v.shape[3]), dtype=torch.bfloat16, device=q.device)
     _call("xfh_sequence_attention", q, k, v, out, lse, low, slopes, masks, options)
     return out, lse, low
