@@ -344,3 +344,60 @@ def test_second_backward_is_refused(device):
     (dq,) = torch.autograd.grad(fastnn.sequence_attention(q, k, v).sum(), [q], create_graph=True)
     with pytest.raises(RuntimeError):
         dq.sum().backward()
+
+
+SPLIT = [  # B, H, Hk, Nq, Nk, D: few work items, so keys, heads and queries are split and joined
+    (1, 2, 1, 1, 2100, 48), (2, 4, 2, 7, 1500, 128), (1, 3, 1, 40, 3000, 33), (1, 1, 1, 200, 1100, 64), (1, 4, 1, 600, 600, 24),
+    (1, 2, 2, 700, 700, 96),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", SPLIT, ids=lambda s: "x".join(map(str, s)))
+def test_split_work(device, shape, dtype):
+    B, H, Hk, nq, nk, D = shape
+    q, k, v, dout = data(device, dtype, *shape, seed=nq)
+    compare(q, k, v, dout, f"split {shape} {dtype}", causal=True, softcap=25.0)
+    docs = documents("packed", nk).to(device)
+    compare(q, k, v, dout, f"split {shape} {dtype} documents", documents=docs,
+            slopes=torch.linspace(0.0, 0.02, H, device=device))
+    lengths = torch.tensor([nk // 3, 0][:B], dtype=torch.int32, device=device)
+    got = compare(q, k, v, dout, f"split {shape} {dtype} lengths", causal=True, lengths=lengths)
+    if B > 1:
+        assert not got["out"][1].any() and not got["dk"][1].any()
+    # a NaN that only the last query's documents hide
+    docs = torch.zeros(nk, dtype=torch.int32, device=device)
+    docs[nk // 2] = 5
+    want = run(q, k, v, dout, causal=True, documents=docs)
+    rest = torch.arange(nk, device=device) != nk // 2
+    for t in (k, v):
+        t[:, :, nk // 2] = math.nan
+    got = run(q, k, v, dout, causal=True, documents=docs)
+    own = rest[nk - nq:]
+    assert torch.equal(got["out"][:, :, own], want["out"][:, :, own]) and torch.equal(got["dq"][:, :, own], want["dq"][:, :, own])
+    for name in ("dk", "dv"):
+        assert torch.equal(got[name][:, :, rest], want[name][:, :, rest]), name
+
+
+def test_two_calls_at_once(device):
+    """Calls of two threads on streams of their own, and of one thread on two streams, with split work."""
+    import threading
+    cases = [data(device, BF16, 1, 4, 1, 300, 900, 64, seed=s) for s in (1, 2)]
+    kw = dict(causal=True, softcap=10.0)
+    want = [run(*c, **kw) for c in cases]
+    torch.cuda.synchronize()
+    got, streams = [None, None], [torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(5):
+                got[i] = run(*cases[i], **kw)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        for name in want[i]:
+            assert torch.equal(got[i][name], want[i][name]), name

@@ -322,8 +322,8 @@ struct SequenceArgs {
 // dv of the heads that share a key and of their queries. The parts are joined in their order.
 struct Splits { int heads, tiles; };
 struct SequenceSplits { int keys; Splits queries; };
-// Parts of a forward pass: (running maximum, sum) and o [splits][B Hk][columns][Dv], columns query by query over
-// the heads of a key head.
+// Parts of a forward pass: (running maximum, sum) and o [splits][B Hk][columns][Dv],
+// columns query by query over the heads of a key head. A part whose sum is 0 has no o.
 struct Parts {
   float2 *ml;
   float *o;

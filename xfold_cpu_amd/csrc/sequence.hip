@@ -364,6 +364,7 @@ __global__ __launch_bounds__(256) void forward_kernel(SequenceArgs a, int blocks
   if (parts.splits > 1) {
     const int64_t at = (int64_t(own.split) * a.B * a.Hk + int64_t(b) * a.Hk + hk) * (a.H / a.Hk * a.Nq) + own.c;
     if (grp == 0) parts.ml[at] = make_float2(m, l);
+    if (l == 0.f) return;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t)
 #pragma unroll
@@ -404,6 +405,7 @@ template <typename T, int N> __global__ __launch_bounds__(256) void join_kernel(
   for (int e = 0; e < N; ++e) v[e] = 0.f;
   for (int s = 0; s < parts.splits; ++s) {
     const float2 p = parts.ml[s * total + column];
+    if (p.y == 0.f) continue;
     const float f = weight_of<T>(p.x, top);
     float o[N];
     __builtin_memcpy(o, __builtin_assume_aligned(parts.o + (s * total + column) * a.Dv + d, 4 * N), 4 * N);
@@ -768,7 +770,9 @@ SequenceSplits sequence_splits(const SequenceArgs &a, int dtype) {
   const int64_t columns = int64_t(a.H / a.Hk) * a.Nq, single = int64_t(a.B) * a.Hk;
   if (columns > 0 && a.Nk > 0) {
     // Keys are split until there are about 512 work items (two workgroups per CU), down to 8 tiles each, 4 of
-    // single tokens. 4 x 200 queries of 5000 keys in bf16: 77 + 9 us in two splits (224 work items unsplit), 115 in one.
+    // single tokens, each sequence in equal parts. 4 x 200 queries of up to 5000 keys in bf16 (224 work items): 115 us
+    // in one part, 68 + 9 in two, 97 + 13 in up to four of 20 tiles: a second round of workgroups costs more than
+    // the shorter sequences' idle ones.
     const int64_t items = columns <= 32 ? single : single * ceil_div(columns, int64_t(bf ? 128 : kTile));
     const int64_t most = ceil_div(int64_t(a.Nk), int64_t(columns <= 32 ? 256 : 512));
     n.keys = int(std::max(int64_t(1), std::min(std::min(most, 512 / items), int64_t(64))));

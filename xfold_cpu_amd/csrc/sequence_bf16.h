@@ -191,22 +191,24 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("" ::: "memory");
 }
 
-// How a score comes from a dot product: MODE bit 0 = cap, bit 1 = the general form without a cap (distance
-// slopes, or a scale that is not positive). Scores are in log 2 units; with MODE 0 what is held is the
-// dot product, and `unit` = scale log2 e goes into the exponent's multiply-add.
+// How a score comes from a dot product: MODE bit 0 = cap, bit 1 = distance slopes (or a scale that is not
+// positive). Scores are in log 2 units. Without slopes what is held is something that rises with the score,
+// score = unit w + offset, and the exponent's multiply-add does the rest: the dot product itself (MODE 0),
+// or (tanh - 1) / 2 = -1 / (exp(2 x / cap) + 1).
 template <int MODE> struct Score {
-  static constexpr bool CAP = MODE & 1, SLOPE = MODE & 2, RAW = MODE == 0;
-  float unit, to_exponent, cap2, slope;
+  static constexpr bool CAP = MODE & 1, SLOPE = MODE & 2;
+  float unit, offset, to_exponent, cap2, slope;
   __device__ __forceinline__ Score(const SequenceArgs &a, int h)
-      : unit(a.scale * kLog2e), to_exponent(CAP ? a.scale * 2.0f * kLog2e / a.cap : 0.f), cap2(a.cap * kLog2e),
+      : unit(MODE == 1 ? 2.0f * a.cap * kLog2e : a.scale * kLog2e), offset(a.cap * kLog2e),
+        to_exponent(CAP ? a.scale * 2.0f * kLog2e / a.cap : 0.f), cap2(a.cap * kLog2e),
         slope(SLOPE && a.slopes ? a.slopes[h] * kLog2e : 0.f) {}
   // gap = p_i - j; `bent` (1 - tanh^2) when asked for.
   __device__ __forceinline__ float operator()(float dot, float gap, float *bent = nullptr) const {
     float w = dot;
     if constexpr (CAP) {
-      const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * to_exponent) + 1.0f);   // (1 - tanh) / 2
-      w = __builtin_fmaf(r, -2.0f * cap2, cap2);
-      if (bent) *bent = 4.0f * r * (1.0f - r);
+      w = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(dot * to_exponent));
+      if (bent) *bent = -4.0f * __builtin_fmaf(w, w, w);
+      if constexpr (SLOPE) w = __builtin_fmaf(w, 2.0f * cap2, cap2);
     } else if constexpr (SLOPE) {
       w = dot * unit;
     }
@@ -215,9 +217,11 @@ template <int MODE> struct Score {
   }
   // exp2(score - m)
   __device__ __forceinline__ float weight(float w, float m) const {
-    return __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(w, unit, -m) : w - m);
+    return __builtin_amdgcn_exp2f(SLOPE ? w - m : __builtin_fmaf(w, unit, MODE == 1 ? offset - m : -m));
   }
-  __device__ __forceinline__ float in_log2(float w) const { return RAW ? w * unit : w; }
+  __device__ __forceinline__ float in_log2(float w) const {
+    return SLOPE ? w : MODE == 1 ? __builtin_fmaf(w, unit, offset) : w * unit;
+  }
 };
 
 // What a wavefront looks up to hide pairs: bounds and documents of the rows of a tile, in LDS of its own (a

@@ -158,6 +158,7 @@ __global__ __launch_bounds__(256, 2) void forward_bf16_kernel(SequenceArgs a, in
   if (parts.splits > 1) {
     const int64_t at = (int64_t(split) * a.B * a.Hk + int64_t(b) * a.Hk + hk) * columns + c;
     if (ln.half == 0) parts.ml[at] = make_float2(m, l);
+    if (l == 0.f) return;
     float *out = parts.o + at * a.Dv;
 #pragma unroll
     for (int t = 0; t < D::DT; ++t)
@@ -280,7 +281,7 @@ __global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, int 
     const int query = col / group, head = hk * group + col % group;
     if (parts.splits > 1) {
       const int64_t p = (int64_t(split) * a.B * a.Hk + int64_t(b) * a.Hk + hk) * columns + col;
-      parts.o[p * a.Dv + d] = value;
+      if (sum != 0.f) parts.o[p * a.Dv + d] = value;
       if (d == 0) parts.ml[p] = make_float2(top, sum);
     } else {
       const float x = sum == 0.f ? 0.f : value / sum;
