@@ -467,7 +467,7 @@ typedef struct XfhSequenceAttention {
   const int32_t *documents;        /* [batch][keys] (row stride documents_stride), or NULL */
   const int32_t *lengths;          /* [batch], or NULL: every entry has `keys` keys */
   const void *dout;                /* backward: as out */
-  void *dq, *dk, *dv;              /* backward: as q, k, v */
+  void *dq, *dk, *dv;              /* backward: as q, k, v; dk and dv may both be NULL */
   float *dslopes;                  /* backward: fp32 [heads], or NULL */
   int64_t batch, heads, kv_heads, queries, keys, dim, value_dim;
   int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3];

@@ -230,6 +230,20 @@ def test_unbatched_and_no_gradient(device, dtype):
     assert torch.equal(dk, run(q, k, v, dout, causal=True)["dk"])
 
 
+def test_only_what_is_asked_for(device):
+    q, k, v, dout = data(device, BF16, 1, 4, 2, 100, 100, 32)
+    slopes = torch.tensor([0.1, 0.0, 0.2, 0.3], device=device)
+    from xfold_cpu_amd import fastnn
+    want = run(q, k, v, dout, causal=True, slopes=slopes)
+    t = {"q": q, "k": k, "v": v, "slopes": slopes}
+    for name in t:
+        leaf = t[name].detach().requires_grad_()
+        kw = {**t, name: leaf}
+        out = fastnn.sequence_attention(kw["q"], kw["k"], kw["v"], causal=True, slopes=kw["slopes"])
+        (g,) = torch.autograd.grad(out, [leaf], dout)
+        assert torch.equal(g, want["d" + name]), name
+
+
 def test_empty(device):
     from xfold_cpu_amd import fastnn
     for shape in [(0, 2, 1, 5, 5, 8), (2, 2, 1, 0, 5, 8), (2, 2, 1, 5, 0, 8), (1, 0, 1, 5, 5, 8)]:

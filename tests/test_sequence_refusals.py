@@ -72,7 +72,7 @@ def arguments(**change):
     (dict(kv_heads=0), "multiple"), (dict(batch=-1), "31 bits"), (dict(keys=2 ** 31), "31 bits"),
     (dict(queries=9, causal=1), "more queries"), (dict(queries=9, lengths=FAKE), "more queries"),
     (dict(prefix_all=1), "prefix"), (dict(prefix=FAKE), "prefix"), (dict(scale=float("inf")), "finite"),
-    (dict(softcap=float("nan")), "finite"), (dict(q=None), "null"), (dict(v=None), "null"), (dict(out=None), "null"),
+    (dict(softcap=float("nan")), "finite"), (dict(softcap=1e-40), "softcap too small"), (dict(q=None), "null"), (dict(v=None), "null"), (dict(out=None), "null"),
 ])
 def test_library_refuses(change, match):
     args = arguments(**change)
@@ -94,6 +94,8 @@ def test_library_refuses_workspaces_and_missing_gradients():
     assert lib.xfh_sequence_attention_backward(ctypes.addressof(args), FAKE, need - 1, None) == 3
     with pytest.raises(ValueError, match="null"):
         nh.call("xfh_sequence_attention_backward", ctypes.addressof(arguments(lse=None)), FAKE, 1 << 20, None)
+    with pytest.raises(ValueError, match="null"):
+        nh.call("xfh_sequence_attention_backward", ctypes.addressof(arguments(dk=None)), FAKE, 1 << 20, None)
     with pytest.raises(ValueError, match="no slopes"):
         nh.call("xfh_sequence_attention_backward", ctypes.addressof(arguments(dslopes=FAKE)), FAKE, 1 << 20, None)
     assert lib.xfh_sequence_attention_workspace_size(ctypes.addressof(arguments(dim=200))) == -1

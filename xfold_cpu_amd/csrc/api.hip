@@ -954,6 +954,8 @@ static int sequence_args(const XfhSequenceAttention *p, SequenceArgs &a) {
               "sequence_attention: more queries than keys with a causal, document or length mask");
   XFH_REQUIRE(p->causal || !(p->prefix || p->prefix_all), "sequence_attention: a prefix needs the causal mask");
   XFH_REQUIRE(std::isfinite(p->scale) && std::isfinite(p->softcap), "sequence_attention: scale and softcap must be finite");
+  XFH_REQUIRE(p->softcap <= 0.f || (std::isfinite(1.0f / p->softcap) && std::isfinite(p->scale * 2.0f * kLog2e / p->softcap)),
+              "sequence_attention: softcap too small for scale");
   std::memset(&a, 0, sizeof(a));
   a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.lse = p->lse; a.low = p->dtype == XFH_BF16 ? p->out_low : nullptr; a.slopes = p->slopes;
   a.prefix = p->prefix; a.documents = p->documents; a.lengths = p->lengths;
@@ -1025,7 +1027,7 @@ int xfh_sequence_attention_backward(const XfhSequenceAttention *args, void *work
   XFH_REQUIRE(!args->dslopes || a.slopes, "sequence_attention_backward: no slopes to take a gradient of");
   const bool queries = a.B > 0 && a.H > 0 && a.Nq > 0, keys = a.B > 0 && a.Hk > 0 && a.Nk > 0;
   XFH_REQUIRE(!queries || (a.q && a.out && a.lse && a.dout && a.dq), "sequence_attention_backward: null tensor");
-  XFH_REQUIRE(!keys || (a.k && a.v && a.dk && a.dv), "sequence_attention_backward: null tensor");
+  XFH_REQUIRE(!keys || (a.k && a.v && !a.dk == !a.dv), "sequence_attention_backward: null tensor");
   Carver cv(workspace, workspace_bytes);
   if (sequence_carve(cv, p, a, args->dtype, true, args->dslopes != nullptr) > (workspace ? workspace_bytes : 0))
     return fail(XFH_EWORKSPACE, "sequence_attention_backward: workspace too small (need " + std::to_string(cv.used) + " bytes)");

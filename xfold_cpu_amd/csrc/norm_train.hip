@@ -12,6 +12,7 @@
 // of the grid and keeps its lanes' columns in registers; its row groups are added in LDS, and one
 // row of partial sums per workgroup goes to memory. A second kernel adds these in their order, so
 // that a result does not depend on the order in which workgroups ran (no atomics).
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -167,35 +168,37 @@ template <typename T, typename TO, int LPR, int CH, bool VEC>
 __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
   __shared__ float red[4];
   const int sub = threadIdx.x % LPR, C = a.C;
-  const int64_t row = int64_t(blockIdx.x) * (kThreads / LPR) + threadIdx.x / LPR;
-  if (LPR < 256 && row >= a.rows) return;              // (LPR = 256: the grid is the rows)
-  float v[CH][8], w[CH][8], b[CH][8];
-  load_row<LPR, CH, VEC>(static_cast<const T *>(a.x) + row * a.ldx, C, sub, v);
-  load_param<LPR, CH, VEC>(a.w, a.w_dtype, 1.f, C, sub, w);
-  load_param<LPR, CH, VEC>(a.b, a.b_dtype, 0.f, C, sub, b);
-  float s[1] = {0.f};
+  // (With LPR = 256 a workgroup is at one row, and its barriers are met by all of it.)
+  for (int64_t row = int64_t(blockIdx.x) * (kThreads / LPR) + threadIdx.x / LPR; row < a.rows;
+       row += int64_t(gridDim.x) * (kThreads / LPR)) {
+    float v[CH][8], w[CH][8], b[CH][8];
+    load_row<LPR, CH, VEC>(static_cast<const T *>(a.x) + row * a.ldx, C, sub, v);
+    load_param<LPR, CH, VEC>(a.w, a.w_dtype, 1.f, C, sub, w);
+    load_param<LPR, CH, VEC>(a.b, a.b_dtype, 0.f, C, sub, b);
+    float s[1] = {0.f};
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s[0] += v[c][e];
-  row_sums<LPR, 1>(s, red);
-  const float mean = s[0] / float(C);
-  float q[1] = {0.f};
+      for (int e = 0; e < 8; ++e) s[0] += v[c][e];
+    row_sums<LPR, 1>(s, red);
+    const float mean = s[0] / float(C);
+    float q[1] = {0.f};
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[c][e] -= mean;
-      if (column<LPR, VEC>(sub, c, VEC ? 0 : e) < C) q[0] += v[c][e] * v[c][e];
-    }
-  row_sums<LPR, 1>(q, red);
-  const float rstd = 1.0f / sqrtf(q[0] / float(C) + a.eps);
+      for (int e = 0; e < 8; ++e) {
+        v[c][e] -= mean;
+        if (column<LPR, VEC>(sub, c, VEC ? 0 : e) < C) q[0] += v[c][e] * v[c][e];
+      }
+    row_sums<LPR, 1>(q, red);
+    const float rstd = 1.0f / sqrtf(q[0] / float(C) + a.eps);
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[c][e] = v[c][e] * rstd * w[c][e] + b[c][e];
-  store_row<LPR, CH, VEC>(static_cast<TO *>(a.y) + row * C, C, sub, v);
-  if (a.stats && sub == 0) a.stats[row] = make_float2(mean, rstd);
+      for (int e = 0; e < 8; ++e) v[c][e] = v[c][e] * rstd * w[c][e] + b[c][e];
+    store_row<LPR, CH, VEC>(static_cast<TO *>(a.y) + row * C, C, sub, v);
+    if (a.stats && sub == 0) a.stats[row] = make_float2(mean, rstd);
+  }
 }
 
 // A row's dx (in g) from its x (in h; normalised on return) and dy (in g).
@@ -296,46 +299,48 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
 // the caches as far as they reach), and a second kernel with a thread per column for dw and db.
 template <typename T, typename TO> __global__ __launch_bounds__(kThreads) void norm_forward_wide_kernel(NormArgs a) {
   __shared__ float red[4];
-  const int64_t row = blockIdx.x;
-  const T *x = static_cast<const T *>(a.x) + row * a.ldx;
-  TO *y = static_cast<TO *>(a.y) + row * a.C;
-  float s[1] = {0.f}, q[1] = {0.f};
-  for (int c = threadIdx.x; c < a.C; c += kThreads) s[0] += to_f32(x[c]);
-  row_sums<256, 1>(s, red);
-  const float mean = s[0] / float(a.C);
-  for (int c = threadIdx.x; c < a.C; c += kThreads) {
-    const float d = to_f32(x[c]) - mean;
-    q[0] += d * d;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+    TO *y = static_cast<TO *>(a.y) + row * a.C;
+    float s[1] = {0.f}, q[1] = {0.f};
+    for (int c = threadIdx.x; c < a.C; c += kThreads) s[0] += to_f32(x[c]);
+    row_sums<256, 1>(s, red);
+    const float mean = s[0] / float(a.C);
+    for (int c = threadIdx.x; c < a.C; c += kThreads) {
+      const float d = to_f32(x[c]) - mean;
+      q[0] += d * d;
+    }
+    row_sums<256, 1>(q, red);
+    const float rstd = 1.0f / sqrtf(q[0] / float(a.C) + a.eps);
+    for (int c = threadIdx.x; c < a.C; c += kThreads) {
+      float t = (to_f32(x[c]) - mean) * rstd;
+      if (a.w) t *= load_any(a.w, a.w_dtype, c);
+      if (a.b) t += load_any(a.b, a.b_dtype, c);
+      y[c] = from_f32<TO>(t);
+    }
+    if (a.stats && threadIdx.x == 0) a.stats[row] = make_float2(mean, rstd);
   }
-  row_sums<256, 1>(q, red);
-  const float rstd = 1.0f / sqrtf(q[0] / float(a.C) + a.eps);
-  for (int c = threadIdx.x; c < a.C; c += kThreads) {
-    float t = (to_f32(x[c]) - mean) * rstd;
-    if (a.w) t *= load_any(a.w, a.w_dtype, c);
-    if (a.b) t += load_any(a.b, a.b_dtype, c);
-    y[c] = from_f32<TO>(t);
-  }
-  if (a.stats && threadIdx.x == 0) a.stats[row] = make_float2(mean, rstd);
 }
 
 template <typename T, typename TO> __global__ __launch_bounds__(kThreads) void norm_backward_wide_kernel(NormArgs a) {
   __shared__ float red[8];
-  const int64_t row = blockIdx.x;
-  const T *x = static_cast<const T *>(a.x) + row * a.ldx;
-  const TO *dy = static_cast<const TO *>(a.dy) + row * a.lddy;
-  T *dx = static_cast<T *>(a.dx) + row * a.C;
-  const float2 st = a.stats[row];
-  float s[2] = {0.f, 0.f};
-  for (int c = threadIdx.x; c < a.C; c += kThreads) {
-    const float g = to_f32(dy[c]) * (a.w ? load_any(a.w, a.w_dtype, c) : 1.f);
-    s[0] += g;
-    s[1] += g * (to_f32(x[c]) - st.x) * st.y;
-  }
-  row_sums<256, 2>(s, red);
-  const float mg = s[0] / float(a.C), mgh = s[1] / float(a.C);
-  for (int c = threadIdx.x; c < a.C; c += kThreads) {
-    const float g = to_f32(dy[c]) * (a.w ? load_any(a.w, a.w_dtype, c) : 1.f);
-    dx[c] = from_f32<T>(st.y * (g - mg - (to_f32(x[c]) - st.x) * st.y * mgh));
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+    const TO *dy = static_cast<const TO *>(a.dy) + row * a.lddy;
+    T *dx = static_cast<T *>(a.dx) + row * a.C;
+    const float2 st = a.stats[row];
+    float s[2] = {0.f, 0.f};
+    for (int c = threadIdx.x; c < a.C; c += kThreads) {
+      const float g = to_f32(dy[c]) * (a.w ? load_any(a.w, a.w_dtype, c) : 1.f);
+      s[0] += g;
+      s[1] += g * (to_f32(x[c]) - st.x) * st.y;
+    }
+    row_sums<256, 2>(s, red);
+    const float mg = s[0] / float(a.C), mgh = s[1] / float(a.C);
+    for (int c = threadIdx.x; c < a.C; c += kThreads) {
+      const float g = to_f32(dy[c]) * (a.w ? load_any(a.w, a.w_dtype, c) : 1.f);
+      dx[c] = from_f32<T>(st.y * (g - mg - (to_f32(x[c]) - st.x) * st.y * mgh));
+    }
   }
 }
 
@@ -486,14 +491,14 @@ template <typename T, typename TO> int launch_typed(const NormArgs &a, bool back
   const auto aligned = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   const bool vec = a.C % 8 == 0 && a.ldx % 8 == 0 && (!backward || a.lddy % 8 == 0) && aligned(a.x) && aligned(a.dy) &&
                    aligned(a.w) && aligned(a.b) && aligned(a.y) && aligned(a.dx) && aligned(a.partial);
-  const int64_t blocks = backward ? backward_blocks(a.rows, a.C) : ceil_div(a.rows, int64_t(kThreads / shape.lpr));
-  if (blocks > (int64_t(1) << 31) - 1 || (shape.ch == 0 && a.rows > (int64_t(1) << 31) - 1))
-    return fail(XFH_EUNSUPPORTED, "layer_norm_train: too many rows");
+  constexpr int64_t kMostBlocks = int64_t(1) << 22;     // (a grid holds fewer than 2^32 threads; the rest goes by a stride)
+  const int64_t blocks = backward ? backward_blocks(a.rows, a.C)
+                                  : std::min(ceil_div(a.rows, int64_t(kThreads / shape.lpr)), kMostBlocks);
   if (shape.ch == 0) {
     if (!backward) {
-      norm_forward_wide_kernel<T, TO><<<dim3(unsigned(a.rows)), kThreads, 0, s>>>(a);
+      norm_forward_wide_kernel<T, TO><<<dim3(unsigned(std::min(a.rows, kMostBlocks))), kThreads, 0, s>>>(a);
     } else {
-      if (a.dx) norm_backward_wide_kernel<T, TO><<<dim3(unsigned(a.rows)), kThreads, 0, s>>>(a);
+      if (a.dx) norm_backward_wide_kernel<T, TO><<<dim3(unsigned(std::min(a.rows, kMostBlocks))), kThreads, 0, s>>>(a);
       if (a.partial)
         norm_columns_kernel<T, TO><<<dim3(unsigned(ceil_div(a.C, int64_t(kThreads))), unsigned(blocks)), kThreads, 0, s>>>(a);
     }

@@ -739,7 +739,7 @@ template <typename T, int DP> int launch_backward(const SequenceArgs &a, const S
   const bool vec = vector_rows<T>({{a.k, a.ks}, {a.q, a.qs}}, a.D) && vector_rows<T>({{a.v, a.vs}, {a.dout, a.gs}}, a.Dv);
   if (qblocks > 0) dq_kernel<T, DP><<<dim3(unsigned(qblocks * a.Hk * a.B)), 256, 0, s>>>(a, int(qblocks), vec);
   XFH_TRY(check_launch("sequence_attention_backward"));
-  if (kblocks > 0)
+  if (kblocks > 0 && (a.dk || a.dv))
     dkv_kernel<T, DP><<<dim3(unsigned(kblocks * a.Hk * a.B * splits.heads * splits.tiles)), 256, 0, s>>>(a, splits, parts, vec);
   return check_launch("sequence_attention_backward");
 }
@@ -747,7 +747,9 @@ template <typename T, int DP> int launch_backward(const SequenceArgs &a, const S
 int check_grid(const SequenceArgs &a) {
   // At most 64 splits of a work item's keys, and those only of few work items.
   const int64_t most = std::max((ceil_div(int64_t(a.Nq), int64_t(kTile)) + 1) * a.H, ceil_div(int64_t(a.Nk), int64_t(kTile)) * a.Hk) * a.B;
-  if (most > (int64_t(1) << 31) - 65536 || int64_t(a.H / std::max(a.Hk, 1)) * a.Nq > (int64_t(1) << 31) - 256) return fail(XFH_EUNSUPPORTED, "sequence_attention: problem too large");
+  // (A grid holds fewer than 2^32 threads.)
+  if (most > (int64_t(1) << 24) - 65536 || int64_t(a.H / std::max(a.Hk, 1)) * a.Nq > (int64_t(1) << 31) - 256)
+    return fail(XFH_EUNSUPPORTED, "sequence_attention: problem too large");
   return XFH_OK;
 }
 
@@ -848,7 +850,7 @@ int sequence_backward(const SequenceArgs &a, int dtype, void *memory, float *dsl
     else XFH_SEQ_BACKWARD(128);
 #undef XFH_SEQ_BACKWARD
     if (status != XFH_OK) return status;
-    if (count > 1) {
+    if (count > 1 && (a.dk || a.dv)) {
       const bool quads = a.D % 4 == 0 && a.Dv % 4 == 0;
       const dim3 grid(unsigned(ceil_div(int64_t(a.B) * a.Hk * a.Nk * ((a.D + a.Dv) / (quads ? 4 : 1)), int64_t(256))));
       if (dtype == XFH_BF16) {

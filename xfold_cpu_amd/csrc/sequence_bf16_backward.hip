@@ -408,7 +408,7 @@ int sequence_bf16_backward(const SequenceArgs &a, const Splits &splits, float *p
     constexpr int MODE = decltype(mode)::value;
     if (blocks > 0) dq_bf16_kernel<D, MODE><<<dim3(unsigned(blocks * a.Hk * a.B)), 256, 0, s>>>(a, int(blocks));
     XFH_TRY(check_launch("sequence_attention_backward"));
-    if (kblocks > 0)
+    if (kblocks > 0 && (a.dk || a.dv))
       dkv_bf16_kernel<E, MODE><<<dim3(unsigned(kblocks * a.Hk * a.B * splits.heads * splits.tiles)), 256, 0, s>>>(a, splits, parts);
     return check_launch("sequence_attention_backward");
   });

@@ -14,7 +14,6 @@ from torch.autograd.function import once_differentiable
 
 from . import config as fastnn_config
 from . import native_hip as nh
-from . import ops
 
 _NO_STRIDES = (0, 0, 0)
 _CODES = {torch.float32: nh.F32, torch.bfloat16: nh.BF16}
@@ -23,10 +22,17 @@ _PACKED = struct.Struct("15Q33q2f2i")
 assert _PACKED.size == ctypes.sizeof(nh.SequenceAttention)
 
 
+def _cast(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    t = t.contiguous()
+    out = torch.empty(t.shape, dtype=dtype, device=t.device)
+    nh.launch(t.device, "xfh_convert", t.data_ptr(), _CODES[t.dtype], out.data_ptr(), _CODES[dtype], t.numel())
+    return out
+
+
 def _rows(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """``t`` in ``dtype`` with a contiguous last dim (any strides before it)."""
     if t.dtype != dtype:
-        return ops.as_dtype(t, dtype)
+        return _cast(t, dtype)
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
@@ -99,8 +105,10 @@ class _SequenceAttention(torch.autograd.Function):
 def _backward(ctx, dout):
     q, k, v, slopes, out, lse, low, *masks = ctx.saved_tensors
     dout = _rows(dout, q.dtype)
-    dq, dk, dv = (_empty(t, *t.shape[1:]) for t in (q, k, v))
     needs = ctx.needs_input_grad
+    dq, dk, dv = _empty(q, *q.shape[1:]), None, None
+    if needs[1] or needs[2]:
+        dk, dv = _empty(k, *k.shape[1:]), _empty(v, *v.shape[1:])
     dslopes = torch.empty_like(slopes) if needs[3] else None
     _call("xfh_sequence_attention_backward", q, k, v, out, lse, low, slopes, masks, ctx.options, dout, dq, dk, dv, dslopes)
     grads = [dq, dk, dv, dslopes]
@@ -108,7 +116,7 @@ def _backward(ctx, dout):
         if not needs[i]:
             grads[i] = None
         elif grads[i].dtype != dtype:
-            grads[i] = ops.as_dtype(grads[i], dtype)
+            grads[i] = _cast(grads[i], dtype)
     return (*grads, None, None, None, None, None)
 
 
