@@ -168,37 +168,35 @@ template <typename T, typename TO, int LPR, int CH, bool VEC>
 __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
   __shared__ float red[4];
   const int sub = threadIdx.x % LPR, C = a.C;
-  // (With LPR = 256 a workgroup is at one row, and its barriers are met by all of it.)
-  for (int64_t row = int64_t(blockIdx.x) * (kThreads / LPR) + threadIdx.x / LPR; row < a.rows;
-       row += int64_t(gridDim.x) * (kThreads / LPR)) {
-    float v[CH][8], w[CH][8], b[CH][8];
-    load_row<LPR, CH, VEC>(static_cast<const T *>(a.x) + row * a.ldx, C, sub, v);
-    load_param<LPR, CH, VEC>(a.w, a.w_dtype, 1.f, C, sub, w);
-    load_param<LPR, CH, VEC>(a.b, a.b_dtype, 0.f, C, sub, b);
-    float s[1] = {0.f};
+  const int64_t row = int64_t(blockIdx.x) * (kThreads / LPR) + threadIdx.x / LPR;
+  if (LPR < 256 && row >= a.rows) return;              // (LPR = 256: the grid is the rows)
+  float v[CH][8], w[CH][8], b[CH][8];
+  load_row<LPR, CH, VEC>(static_cast<const T *>(a.x) + row * a.ldx, C, sub, v);
+  load_param<LPR, CH, VEC>(a.w, a.w_dtype, 1.f, C, sub, w);
+  load_param<LPR, CH, VEC>(a.b, a.b_dtype, 0.f, C, sub, b);
+  float s[1] = {0.f};
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+  for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[0] += v[c][e];
-    row_sums<LPR, 1>(s, red);
-    const float mean = s[0] / float(C);
-    float q[1] = {0.f};
+    for (int e = 0; e < 8; ++e) s[0] += v[c][e];
+  row_sums<LPR, 1>(s, red);
+  const float mean = s[0] / float(C);
+  float q[1] = {0.f};
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+  for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[c][e] -= mean;
-        if (column<LPR, VEC>(sub, c, VEC ? 0 : e) < C) q[0] += v[c][e] * v[c][e];
-      }
-    row_sums<LPR, 1>(q, red);
-    const float rstd = 1.0f / sqrtf(q[0] / float(C) + a.eps);
+    for (int e = 0; e < 8; ++e) {
+      v[c][e] -= mean;
+      if (column<LPR, VEC>(sub, c, VEC ? 0 : e) < C) q[0] += v[c][e] * v[c][e];
+    }
+  row_sums<LPR, 1>(q, red);
+  const float rstd = 1.0f / sqrtf(q[0] / float(C) + a.eps);
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+  for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[c][e] = v[c][e] * rstd * w[c][e] + b[c][e];
-    store_row<LPR, CH, VEC>(static_cast<TO *>(a.y) + row * C, C, sub, v);
-    if (a.stats && sub == 0) a.stats[row] = make_float2(mean, rstd);
-  }
+    for (int e = 0; e < 8; ++e) v[c][e] = v[c][e] * rstd * w[c][e] + b[c][e];
+  store_row<LPR, CH, VEC>(static_cast<TO *>(a.y) + row * C, C, sub, v);
+  if (a.stats && sub == 0) a.stats[row] = make_float2(mean, rstd);
 }
 
 // A row's dx (in g) from its x (in h; normalised on return) and dy (in g).
@@ -491,9 +489,23 @@ template <typename T, typename TO> int launch_typed(const NormArgs &a, bool back
   const auto aligned = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   const bool vec = a.C % 8 == 0 && a.ldx % 8 == 0 && (!backward || a.lddy % 8 == 0) && aligned(a.x) && aligned(a.dy) &&
                    aligned(a.w) && aligned(a.b) && aligned(a.y) && aligned(a.dx) && aligned(a.partial);
-  constexpr int64_t kMostBlocks = int64_t(1) << 22;     // (a grid holds fewer than 2^32 threads; the rest goes by a stride)
-  const int64_t blocks = backward ? backward_blocks(a.rows, a.C)
-                                  : std::min(ceil_div(a.rows, int64_t(kThreads / shape.lpr)), kMostBlocks);
+  // A grid holds fewer than 2^32 threads: more rows go in several launches (as a stride in the kernel they took 65
+  // in place of 57 us at 589824x128).
+  constexpr int64_t kMostBlocks = int64_t(1) << 22;
+  const int64_t most_rows = kMostBlocks * (kThreads / shape.lpr);
+  if (!backward && shape.ch > 0 && a.rows > most_rows) {
+    for (int64_t row = 0; row < a.rows; row += most_rows) {
+      NormArgs part = a;
+      part.rows = std::min(most_rows, a.rows - row);
+      part.x = static_cast<const T *>(a.x) + row * a.ldx;
+      part.y = static_cast<TO *>(a.y) + row * a.C;
+      if (a.stats) part.stats = a.stats + row;
+      const int status = launch_typed<T, TO>(part, false, p, s);
+      if (status != XFH_OK) return status;
+    }
+    return XFH_OK;
+  }
+  const int64_t blocks = backward ? backward_blocks(a.rows, a.C) : ceil_div(a.rows, int64_t(kThreads / shape.lpr));
   if (shape.ch == 0) {
     if (!backward) {
       norm_forward_wide_kernel<T, TO><<<dim3(unsigned(std::min(a.rows, kMostBlocks))), kThreads, 0, s>>>(a);
