@@ -133,3 +133,9 @@ def test_layer_norm_library_refuses():
     assert need > 0
     assert lib.xfh_layer_norm_backward(f, 0, 64, f, 0, 64, 1000, 64, None, 0, f, f, f, 0, None, 0, f, need - 1, None) == 3
     assert lib.xfh_layer_norm_train(None, 0, 4, 0, 4, None, 0, None, 0, 1e-5, None, 0, None, None) == 0
+
+
+def test_autograd_extension_of_another_abi():
+    with pytest.raises(RuntimeError, match="rebuild"):
+        nh.autograd().bind(nh.ABI_VERSION + 1, {})
+    nh.autograd().bind(nh.ABI_VERSION, {name: ctypes.cast(nh.function(name), ctypes.c_void_p).value for name in nh.SIGNATURES})

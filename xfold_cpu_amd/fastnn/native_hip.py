@@ -21,6 +21,8 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import importlib.machinery
+import importlib.util
 import os
 from pathlib import Path
 from typing import Optional
@@ -170,6 +172,19 @@ def function(name: str):
     return getattr(load_library(), name)
 
 
+@functools.lru_cache(maxsize=None)
+def autograd():
+    """The extension with the autograd nodes (``csrc/autograd.cpp``), bound to the library's functions."""
+    path = LIBRARY_PATH.with_name("xfold_autograd.so")
+    if not path.exists():
+        raise RuntimeError(f"The 'hip' backend needs {path}; build it with `python -m xfold_cpu_amd._build`.")
+    loader = importlib.machinery.ExtensionFileLoader("xfold_autograd", str(path))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("xfold_autograd", loader))
+    loader.exec_module(module)
+    module.bind(ABI_VERSION, {name: ctypes.cast(function(name), ctypes.c_void_p).value for name in SIGNATURES})
+    return module
+
+
 def launch(device: torch.device, name: str, *args) -> None:
     """:func:`call` with ``device`` as the current one and its current stream as the last argument."""
     index = device.index
@@ -248,14 +263,6 @@ def check_gpu(*tensors) -> None:
             index = tensor.get_device()
         elif tensor.get_device() != index:
             raise ValueError(f"The 'hip' backend requires tensors on one device, got cuda:{index} and {tensor.device}.")
-
-
-def needs_gradient(*tensors) -> bool:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
 
 
 def compute_dtype(x: torch.Tensor, *weights: torch.Tensor) -> torch.dtype:
