@@ -415,3 +415,40 @@ def test_two_calls_at_once(device):
     for i in range(2):
         for name in want[i]:
             assert torch.equal(got[i][name], want[i][name]), name
+
+
+RAGGED = [  # H, Hk, Nq, Nk, D, lengths: the sequences share the parts by their lengths
+    (8, 2, 5, 2300, 128, (2300, 17, 0, 900, 1)), (4, 1, 150, 1700, 64, (1, 1700, 64, 1100)),
+    (2, 1, 1, 600, 24, tuple((37 * i) % 601 for i in range(70))), (3, 1, 40, 3000, 33, (3000, 30)),
+    (2, 2, 90, 2100, 96, (0, 0, 0)),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", RAGGED, ids=lambda s: "x".join(map(str, (len(s[5]),) + s[:5])))
+def test_split_sequences_of_different_lengths(device, shape, dtype):
+    H, Hk, nq, nk, D, lengths = shape
+    q, k, v, dout = data(device, dtype, len(lengths), H, Hk, nq, nk, D, seed=nk)
+    lengths = torch.tensor(lengths, dtype=torch.int32, device=device)
+    compare(q, k, v, dout, f"lengths {shape} {dtype}", causal=True, lengths=lengths)
+    compare(q, k, v, dout, f"lengths {shape} {dtype} documents", documents=documents("packed", nk).to(device), lengths=lengths)
+
+
+def test_captured_call_reads_the_lengths_of_its_replay(device):
+    from xfold_cpu_amd import fastnn
+    q, k, v, _ = data(device, BF16, 4, 8, 2, 30, 2000, 64, seed=11)
+    lengths = torch.tensor([2000, 40, 700, 0], dtype=torch.int32, device=device)
+    call = lambda: fastnn.sequence_attention(q, k, v, causal=True, lengths=lengths)           # noqa: E731
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        call()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for now in ((2000, 40, 700, 0), (1, 2000, 2000, 2000), (65, 0, 0, 1999), (2000, 2000, 2000, 2000)):
+        lengths.copy_(torch.tensor(now, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call()), now

@@ -321,13 +321,16 @@ struct SequenceArgs {
 // Parts that a pass is split in where it has few work items: of the keys in the forward pass, and for dk and
 // dv of the heads that share a key and of their queries. The parts are joined in their order.
 struct Splits { int heads, tiles; };
-struct SequenceSplits { int keys; Splits queries; };
-// Parts of a forward pass: (running maximum, sum) and o [splits][B Hk][columns][Dv],
-// columns query by query over the heads of a key head. A part whose sum is 0 has no o.
+// Keys: `keys` parts of each sequence, or, where the sequences have lengths of their own, `slots` parts in all.
+struct SequenceSplits { int keys, slots; Splits queries; };
+// Parts of a forward pass: (running maximum, sum) and o [slots][Hk][columns][Dv],
+// columns query by query over the heads of a key head. A part whose sum is 0 has no o. Part s of sequence b is
+// slot s B + b, or with a table, which the forward kernel writes, slot table[b].x + s of table[b].y.
 struct Parts {
   float2 *ml;
   float *o;
-  int splits;
+  int2 *table;
+  int splits, slots;
 };
 SequenceSplits sequence_splits(const SequenceArgs &a, int dtype);
 int64_t sequence_forward_parts(const SequenceArgs &a, const SequenceSplits &n);     // bytes

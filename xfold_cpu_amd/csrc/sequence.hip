@@ -241,19 +241,15 @@ template <typename T> __device__ __forceinline__ float probability(float x, cons
 // What a workgroup with 64 columns of queries works on: columns and work items are as in the bf16 kernels
 // (sequence_bf16_forward.hip), query by query over the heads that share a key head.
 struct Columns {
-  int b, h, hk, i, split, c;
+  int b, h, hk, i, c;
   bool valid;
   Place place;
   Row row;
   Span span;
-  __device__ __forceinline__ Columns(const SequenceArgs &a, int blocks, int splits) {
-    const int group = a.H / a.Hk, columns = group * a.Nq;
-    hk = blockIdx.x % a.Hk;
-    int rest = blockIdx.x / a.Hk;
-    split = rest % splits;
-    rest /= splits;
-    const int blk = blocks - 1 - rest % blocks;
-    b = rest / blocks;
+  __device__ __forceinline__ Columns(const SequenceArgs &a, const Part &part) {
+    const int group = a.H / a.Hk, columns = group * a.Nq, blk = part.blk;
+    hk = part.hk;
+    b = part.b;
     const int c0 = blk * kTile, c1 = min(c0 + kTile, columns) - 1;
     c = c0 + (threadIdx.x >> 6) * 16 + (threadIdx.x & 15);
     valid = c < columns;
@@ -270,7 +266,9 @@ __global__ __launch_bounds__(256) void forward_kernel(SequenceArgs a, int blocks
   constexpr int P = DP + pitch_pad<T>();
   __shared__ __attribute__((aligned(16))) T ks[kTile * P], vs[kTile * P];
   __shared__ int ids[kTile];
-  const Columns own(a, blocks, parts.splits);
+  const Part part(a, parts, blocks);
+  if (part.count == 0) return;
+  const Columns own(a, part);
   const int b = own.b, h = own.h, hk = own.hk, i = own.i;
   const int tid = threadIdx.x, lane = tid & 63, grp = lane >> 4;
   const Place &place = own.place;
@@ -283,11 +281,7 @@ __global__ __launch_bounds__(256) void forward_kernel(SequenceArgs a, int blocks
   const auto test = [&](int tile) { return key_tile_needs(a, b, tile, own.span, own.span); };
   const Scorer<T> score(a, h);
   int end = (own.span.high + kTile - 1) / kTile, begin = 0;
-  if (parts.splits > 1) {
-    const int per = (end + parts.splits - 1) / parts.splits;
-    begin = min(own.split * per, end);
-    end = min(begin + per, end);
-  }
+  if (several(parts)) part.take(begin, end);
 
   f32x4 o[DP / 16];
   float m, l;
@@ -361,8 +355,8 @@ __global__ __launch_bounds__(256) void forward_kernel(SequenceArgs a, int blocks
   }
   l = column_sum(l);
   if (!valid) return;
-  if (parts.splits > 1) {
-    const int64_t at = (int64_t(own.split) * a.B * a.Hk + int64_t(b) * a.Hk + hk) * (a.H / a.Hk * a.Nq) + own.c;
+  if (several(parts)) {
+    const int64_t at = (int64_t(part.slot) * a.Hk + hk) * (a.H / a.Hk * a.Nq) + own.c;
     if (grp == 0) parts.ml[at] = make_float2(m, l);
     if (l == 0.f) return;
 #pragma unroll
@@ -398,22 +392,48 @@ template <typename T, int N> __global__ __launch_bounds__(256) void join_kernel(
   if (at >= total * pieces) return;
   const int64_t column = at / pieces;
   const int d = int(at - column * pieces) * N;
+  const int c = int(column % columns), bk = int(column / columns), hk = bk % a.Hk, b = bk / a.Hk;
+  int slot = b, step = a.B, count = parts.splits;
+  if (parts.table) {
+    const int2 t = parts.table[b];
+    slot = t.x;
+    step = 1;
+    count = t.y;
+  }
+  const int64_t from = (int64_t(slot) * a.Hk + hk) * columns + c, stride = int64_t(step) * a.Hk * columns;
+  // Four parts at a time, whose loads do not wait for each other (for tokens of 16 sequences of up to 8192 keys forward pass
+  // and join take 62.5 us, 64.3 with one part at a time; eight take more registers: 75 us for 72 in the case at seq::Part).
+  constexpr int kBatch = 4;
   float top = kLowest;
-  for (int s = 0; s < parts.splits; ++s) top = fmaxf(top, parts.ml[s * total + column].x);
+  for (int s = 0; s < count; s += kBatch) {
+    float m[kBatch];
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) m[e] = s + e < count ? parts.ml[from + (s + e) * stride].x : kLowest;
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) top = fmaxf(top, m[e]);
+  }
   float sum = 0.f, v[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) v[e] = 0.f;
-  for (int s = 0; s < parts.splits; ++s) {
-    const float2 p = parts.ml[s * total + column];
-    if (p.y == 0.f) continue;
-    const float f = weight_of<T>(p.x, top);
-    float o[N];
-    __builtin_memcpy(o, __builtin_assume_aligned(parts.o + (s * total + column) * a.Dv + d, 4 * N), 4 * N);
-    sum += f * p.y;
+  for (int s = 0; s < count; s += kBatch) {
+    float2 p[kBatch];
+    float o[kBatch][N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] += f * o[e];
+    for (int j = 0; j < kBatch; ++j) {
+      if (s + j >= count) break;
+      const int64_t row = from + (s + j) * stride;
+      p[j] = parts.ml[row];
+      __builtin_memcpy(o[j], __builtin_assume_aligned(parts.o + row * a.Dv + d, 4 * N), 4 * N);
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (s + j >= count || p[j].y == 0.f) continue;     // (a part whose sum is 0 has no o)
+      const float f = weight_of<T>(p[j].x, top);
+      sum += f * p[j].y;
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] += f * o[j][e];
+    }
   }
-  const int c = int(column % columns), bk = int(column / columns), hk = bk % a.Hk, b = bk / a.Hk;
   const int i = c / group, h = hk * group + c % group;
   const int64_t row = (int64_t(b) * a.H + h) * a.Nq + i;
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
@@ -443,7 +463,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
   constexpr int P = DP + pitch_pad<T>();
   __shared__ __attribute__((aligned(16))) T ks[kTile * P], vs[kTile * P];
   __shared__ int ids[kTile];
-  const Columns own(a, blocks, 1);
+  const Columns own(a, Part(a, Parts{nullptr, nullptr, nullptr, 1, a.B}, blocks));
   const int b = own.b, h = own.h, hk = own.hk, i = own.i;
   const int tid = threadIdx.x, lane = tid & 63, grp = lane >> 4;
   const Place &place = own.place;
@@ -730,7 +750,7 @@ template <typename T> bool vector_rows(std::initializer_list<std::pair<const voi
 template <typename T, int DP> int launch_forward(const SequenceArgs &a, const Parts &parts, hipStream_t s) {
   const int64_t blocks = ceil_div(int64_t(a.H / a.Hk) * a.Nq, int64_t(kTile));
   const bool vec = vector_rows<T>({{a.q, a.qs}, {a.k, a.ks}}, a.D) && vector_rows<T>({{a.v, a.vs}}, a.Dv);
-  forward_kernel<T, DP><<<dim3(unsigned(blocks * a.Hk * a.B * parts.splits)), 256, 0, s>>>(a, int(blocks), parts, vec);
+  forward_kernel<T, DP><<<dim3(unsigned(blocks * a.Hk * parts.slots)), 256, 0, s>>>(a, int(blocks), parts, vec);
   return check_launch("sequence_attention");
 }
 
@@ -765,19 +785,28 @@ int sequence_ranges(const SequenceArgs &a, hipStream_t s) {
   return check_launch("sequence_attention");
 }
 
+// Whether the parts are distributed by the sequences' lengths, which only the device has (seq::Part).
+static bool shares_slots(const SequenceArgs &a) { return a.lengths && a.B > 1 && int64_t(a.H / a.Hk) * a.Nq > 32; }
+
 SequenceSplits sequence_splits(const SequenceArgs &a, int dtype) {
-  SequenceSplits n{1, {1, 1}};
+  SequenceSplits n{1, a.B, {1, 1}};
   if (a.B == 0 || a.H == 0 || a.Hk == 0) return n;
   const bool bf = dtype == XFH_BF16 && sequence_bf16_forward_fits(a);
   const int64_t columns = int64_t(a.H / a.Hk) * a.Nq, single = int64_t(a.B) * a.Hk;
   if (columns > 0 && a.Nk > 0) {
-    // Keys are split until there are about 512 work items (two workgroups per CU), down to 8 tiles each, 4 of
-    // single tokens, each sequence in equal parts. 4 x 200 queries of up to 5000 keys in bf16 (224 work items): 115 us
-    // in one part, 68 + 9 in two, 97 + 13 in up to four of 20 tiles: a second round of workgroups costs more than
-    // the shorter sequences' idle ones.
-    const int64_t items = columns <= 32 ? single : single * ceil_div(columns, int64_t(bf ? 128 : kTile));
-    const int64_t most = ceil_div(int64_t(a.Nk), int64_t(columns <= 32 ? 256 : 512));
-    n.keys = int(std::max(int64_t(1), std::min(std::min(most, 512 / items), int64_t(64))));
+    // Keys are split until there are about 512 work items (two workgroups per CU), down to 8 tiles each: 4 x 200
+    // queries of up to 5000 keys in bf16 (224 work items) take 124 us in one part each. Sequences with lengths of
+    // their own share the parts by need (seq::Part). Up to 32 columns (single tokens): down to 4 tiles, in equal
+    // parts. Their workgroups fill a CU's LDS at D = 128: 256 parts, all at once, take 97 us for 16 tokens of 8192 keys (8 key
+    // heads) and 101 for one of 100000, 512 take 106 and 134. With lengths 512, so that a CU with a short part takes
+    // another: 16 of 700 to 8192 keys 63 us against 70 with 256, and 66 to 71 with parts by need.
+    const bool tokens = columns <= 32;
+    const int64_t items = tokens ? single : single * ceil_div(columns, int64_t(bf ? 128 : kTile));
+    const int64_t most = std::min(ceil_div(int64_t(a.Nk), int64_t(tokens ? 256 : 512)), int64_t(64));
+    const int64_t want = tokens && !a.lengths ? 256 : 512;
+    n.keys = int(std::max(int64_t(1), std::min(most, want / items)));
+    n.slots = n.keys * a.B;
+    if (shares_slots(a)) n.slots = int(std::max(int64_t(a.B), std::min(most * a.B, want * a.B / items)));
   }
   if (a.Nk > 0 && a.Nq > 0) {
     // dk and dv are summed in parts (heads first, then runs of queries of at least 4 tiles) until there are about 1024
@@ -790,8 +819,8 @@ SequenceSplits sequence_splits(const SequenceArgs &a, int dtype) {
   return n;
 }
 int64_t sequence_forward_parts(const SequenceArgs &a, const SequenceSplits &n) {
-  const int64_t rows = n.keys * int64_t(a.B) * a.H * a.Nq;
-  return n.keys <= 1 ? 0 : align_up(rows, 2) * 8 + rows * a.Dv * 4;
+  const int64_t rows = int64_t(n.slots) * a.H * a.Nq;
+  return n.slots <= a.B ? 0 : align_up(rows, 2) * 8 + align_up(rows * a.Dv, 2) * 4 + (shares_slots(a) ? int64_t(a.B) * 8 : 0);
 }
 int64_t sequence_backward_parts(const SequenceArgs &a, const SequenceSplits &n) {
   const int64_t count = int64_t(n.queries.heads) * n.queries.tiles;
@@ -802,9 +831,15 @@ int sequence_forward(const SequenceArgs &a, int dtype, void *memory, hipStream_t
   if (a.B == 0 || a.H == 0 || a.Nq == 0) return XFH_OK;
   XFH_TRY(check_grid(a));
   XFH_TRY(sequence_ranges(a, s));
-  const int splits = sequence_splits(a, dtype).keys;
-  Parts parts{static_cast<float2 *>(memory), nullptr, splits};
-  if (splits > 1) parts.o = reinterpret_cast<float *>(parts.ml + align_up(splits * int64_t(a.B) * a.H * a.Nq, 2));   // (on 16 bytes)
+  const SequenceSplits n = sequence_splits(a, dtype);
+  Parts parts{static_cast<float2 *>(memory), nullptr, nullptr, 1, a.B};
+  if (n.slots > a.B) {
+    const int64_t rows = int64_t(n.slots) * a.H * a.Nq;
+    parts.o = reinterpret_cast<float *>(parts.ml + align_up(rows, 2));   // (on 16 bytes)
+    if (shares_slots(a)) parts.table = reinterpret_cast<int2 *>(parts.o + align_up(rows * a.Dv, 2));
+    else parts.splits = n.keys;
+    parts.slots = n.slots;
+  }
   if (dtype == XFH_BF16 && sequence_bf16_forward_fits(a)) {
     XFH_TRY(sequence_bf16_forward(a, parts, s));
   } else {
@@ -818,7 +853,7 @@ int sequence_forward(const SequenceArgs &a, int dtype, void *memory, hipStream_t
 #undef XFH_SEQ_FORWARD
     if (status != XFH_OK) return status;
   }
-  if (splits <= 1) return XFH_OK;
+  if (n.slots <= a.B) return XFH_OK;
   const bool quads = a.Dv % 4 == 0;
   const dim3 grid(unsigned(ceil_div(int64_t(a.B) * a.H * a.Nq * (quads ? a.Dv / 4 : a.Dv), int64_t(256))));
   if (dtype == XFH_BF16) {

@@ -121,11 +121,9 @@ __global__ __launch_bounds__(256, 2) void forward_bf16_kernel(SequenceArgs a, in
   __shared__ __attribute__((aligned(1024))) bf16 stage0[2 * TILE], stage1[2 * TILE];
   __shared__ __attribute__((aligned(16))) Marks marks[4];
   const int group = a.H / a.Hk, columns = group * a.Nq;
-  const int hk = blockIdx.x % a.Hk;
-  int rest = blockIdx.x / a.Hk;
-  const int split = rest % parts.splits;
-  rest /= parts.splits;
-  const int blk = blocks - 1 - rest % blocks, b = rest / blocks;   // the last queries, which see most under a causal mask, first
+  const Part part(a, parts, blocks);
+  if (part.count == 0) return;
+  const int b = part.b, hk = part.hk, blk = part.blk;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Lane<D> ln;
   const int c0 = blk * kColumns, c1 = min(c0 + kColumns, columns) - 1;
@@ -143,11 +141,7 @@ __global__ __launch_bounds__(256, 2) void forward_bf16_kernel(SequenceArgs a, in
   const Loader<D, 4> kl(static_cast<const bf16 *>(a.k) + b * a.ks[0] + hk * a.ks[1], a.ks[2], place.n, a.D, wave);
   const Loader<D, 4> vl(static_cast<const bf16 *>(a.v) + b * a.vs[0] + hk * a.vs[1], a.vs[2], place.n, a.Dv, wave);
   int end = (block.high + kTile - 1) / kTile, first = 0;
-  if (parts.splits > 1) {
-    const int per = (end + parts.splits - 1) / parts.splits;
-    first = min(split * per, end);
-    end = min(first + per, end);
-  }
+  if (several(parts)) part.take(first, end);
   f32x16 o[D::DT];
   float m, l;
   forward_walk<D, MODE, false>(a, ln, stage0, stage1, kl, vl, qf, score, b, first, end, place.n, block, mine, row, marks[wave], m, l, o);
@@ -155,8 +149,8 @@ __global__ __launch_bounds__(256, 2) void forward_bf16_kernel(SequenceArgs a, in
     forward_walk<D, MODE, true>(a, ln, stage0, stage1, kl, vl, qf, score, b, first, end, place.n, block, mine, row, marks[wave], m, l, o);
   l += other_half(l);
   if (!valid) return;
-  if (parts.splits > 1) {
-    const int64_t at = (int64_t(split) * a.B * a.Hk + int64_t(b) * a.Hk + hk) * columns + c;
+  if (several(parts)) {
+    const int64_t at = (int64_t(part.slot) * a.Hk + hk) * columns + c;
     if (ln.half == 0) parts.ml[at] = make_float2(m, l);
     if (l == 0.f) return;
     float *out = parts.o + at * a.Dv;
@@ -226,7 +220,7 @@ __device__ __forceinline__ void token_walk(const SequenceArgs &a, const Lane<D> 
 }
 
 template <class D, int MODE>
-__global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, int blocks, Parts parts) {
+__global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, Parts parts) {
   constexpr int TILE = 32 * D::DL, PITCH = D::DT * 32 + 4;
   __shared__ __attribute__((aligned(1024))) bf16 stage0[4][2 * TILE], stage1[4][2 * TILE];
   __shared__ __attribute__((aligned(16))) Marks marks[4];
@@ -234,9 +228,8 @@ __global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, int 
   static_assert(sizeof(stage0) >= 2 * 32 * PITCH * 4, "two wavefronts' results are joined in a stage");
   const auto joined = [&](int w) { return reinterpret_cast<float *>(w < 2 ? stage0 : stage1) + (w & 1) * 32 * PITCH; };
   const int group = a.H / a.Hk, columns = group * a.Nq;
-  const int hk = blockIdx.x % a.Hk;
-  int rest = blockIdx.x / a.Hk;
-  const int split = rest % parts.splits, b = rest / parts.splits;
+  const Part part(a, parts, 1);
+  const int b = part.b, hk = part.hk;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Lane<D> ln;
   const int c = ln.col;
@@ -250,8 +243,8 @@ __global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, int 
   own_row<D>(qf, static_cast<const bf16 *>(a.q) + b * a.qs[0] + h * a.qs[1] + i * a.qs[2], a.D, valid, ln.half);
   const Loader<D, 1, 32> kl(static_cast<const bf16 *>(a.k) + b * a.ks[0] + hk * a.ks[1], a.ks[2], place.n, a.D, 0);
   const Loader<D, 1, 32> vl(static_cast<const bf16 *>(a.v) + b * a.vs[0] + hk * a.vs[1], a.vs[2], place.n, a.Dv, 0);
-  const int tiles = (span.high + 31) / 32, per = (tiles + parts.splits - 1) / parts.splits;
-  const int first = min(split * per, tiles), end = min(first + per, tiles);
+  int first, end = (span.high + 31) / 32;
+  part.take(first, end);
   f32x16 o[D::DT];
   float m, l;
   token_walk<D, MODE, false>(a, ln, stage0[wave], stage1[wave], kl, vl, qf, score, b, first + wave, end, place.n, span, row, marks[wave], m, l, o);
@@ -279,8 +272,8 @@ __global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, int 
       value += f * joined(w)[col * PITCH + d];
     }
     const int query = col / group, head = hk * group + col % group;
-    if (parts.splits > 1) {
-      const int64_t p = (int64_t(split) * a.B * a.Hk + int64_t(b) * a.Hk + hk) * columns + col;
+    if (several(parts)) {
+      const int64_t p = (int64_t(part.slot) * a.Hk + hk) * columns + col;
       if (sum != 0.f) parts.o[p * a.Dv + d] = value;
       if (d == 0) parts.ml[p] = make_float2(top, sum);
     } else {
@@ -304,11 +297,11 @@ bool sequence_bf16_forward_fits(const SequenceArgs &a) {
 int sequence_bf16_forward(const SequenceArgs &a, const Parts &parts, hipStream_t s) {
   const int64_t columns = int64_t(a.H / a.Hk) * a.Nq;
   const int64_t blocks = columns <= 32 ? 1 : ceil_div(columns, int64_t(kColumns));
-  const dim3 grid(unsigned(blocks * a.Hk * a.B * parts.splits));
+  const dim3 grid(unsigned(blocks * a.Hk * parts.slots));
   return with_dims(a, [&](auto dim, auto mode) {
     typedef decltype(dim) D;
     constexpr int MODE = decltype(mode)::value;
-    if (columns <= 32) token_bf16_kernel<D, MODE><<<grid, 256, 0, s>>>(a, 1, parts);
+    if (columns <= 32) token_bf16_kernel<D, MODE><<<grid, 256, 0, s>>>(a, parts);
     else forward_bf16_kernel<D, MODE><<<grid, 256, 0, s>>>(a, int(blocks), parts);
     return check_launch("sequence_attention");
   });
