@@ -177,6 +177,22 @@ def test_graph_replays_and_streams(device):
             assert torch.equal(got[name], want[name]), (seed, name)
 
 
+def test_more_rows_than_a_launch(device):
+    from xfold_cpu_amd import fastnn
+    rows, C = (1 << 26) + 5, 2
+    x = torch.empty(rows, C, dtype=BF16, device=device).copy_((torch.arange(rows, device=device) % 253)[:, None])
+    x[:, 1] -= (torch.arange(rows, device=device) % 7).to(BF16)
+    w, b = torch.tensor([1.5, -0.5], device=device), torch.tensor([0.25, 4.0], device=device)
+    for part in (slice(0, 100), slice((1 << 26) - 50, (1 << 26) + 5)):
+        leaf, some = x.detach().requires_grad_(), x[part].detach().requires_grad_()
+        y, want = fastnn.trainable_layer_norm(leaf, (C,), w, b), fastnn.trainable_layer_norm(some, (C,), w, b)
+        assert torch.equal(y[part], want)
+        dy = torch.zeros_like(y)
+        dy[part] = torch.tensor([1.0, 3.0], dtype=BF16, device=device)
+        (dx,), (want,) = torch.autograd.grad(y, leaf, dy), torch.autograd.grad(want, some, dy[part])
+        assert torch.equal(dx[part], want)
+
+
 # ------------------------------------------------------------------------------ the operators together
 
 class Block(torch.nn.Module):
@@ -230,3 +246,39 @@ def test_pre_norm_attention_block(device):
         # FP32 throughout: five products in a row over at most 180 terms, each 180 * 2^-24 = 1e-5 of its
         # absolute terms at most; errors add at random, but the norms of sums are smaller than their terms'.
         assert err <= 5e-5, (name, err)
+
+
+def test_checkpointed_block(device):
+    """Recomputed in the backward pass, with hooks on the saved tensors: the same bits."""
+    from torch.utils.checkpoint import checkpoint
+    from xfold_cpu_amd import fastnn
+    torch.manual_seed(1)
+    block = Block(fastnn.LayerNorm(96), fastnn.sequence_attention).to(device).train()
+    x = torch.randn(2, 70, 96, device=device, requires_grad=True)
+    leaves = [x, *block.parameters()]
+    call = lambda t: block(t, causal=True, softcap=12.0)                                              # noqa: E731
+    want = torch.autograd.grad(call(x).square().sum(), leaves)
+    got = torch.autograd.grad(checkpoint(call, x, use_reentrant=False).square().sum(), leaves)
+    with torch.autograd.graph.save_on_cpu():
+        moved = torch.autograd.grad(call(x).square().sum(), leaves)
+    for w, g, m in zip(want, got, moved):
+        assert torch.equal(w, g) and torch.equal(w, m)
+
+
+def test_gradients_of_two_graphs_and_of_some_inputs(device):
+    """One graph differentiated twice, and for one input at a time: what is not asked for is left out."""
+    x, w, b, dy = data(device, BF16, F32, 300, 96)
+    want = run(x, w, b, dy)
+    from xfold_cpu_amd import fastnn
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    y = fastnn.trainable_layer_norm(leaves[0], (96,), *leaves[1:])
+    for _ in range(2):
+        for name, leaf in zip(("dx", "dw", "db"), leaves):
+            (g,) = torch.autograd.grad(y, leaf, dy, retain_graph=True)
+            assert torch.equal(g, want[name]), name
+    y = fastnn.trainable_layer_norm(leaves[0], (96,), None, leaves[2])          # no weight: the bias keeps its place
+    gx, gb = torch.autograd.grad(y, (leaves[0], leaves[2]), dy)
+    assert torch.equal(gb, want["db"]) and gx.shape == x.shape
+    (twice,) = torch.autograd.grad(fastnn.trainable_layer_norm(leaves[0], (96,)).sum(), leaves[0], create_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        twice.sum().backward()
