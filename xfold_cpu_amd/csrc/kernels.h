@@ -337,6 +337,16 @@ int64_t sequence_forward_parts(const SequenceArgs &a, const SequenceSplits &n); 
 int64_t sequence_backward_parts(const SequenceArgs &a, const SequenceSplits &n);
 int64_t sequence_ranges_bytes(int64_t B, int64_t Nk);
 int64_t sequence_slope_part(int64_t B, int64_t H, int64_t Nq);   // floats
+constexpr int64_t kMostItems = (int64_t(1) << 24) - 65536;       // (a grid holds fewer than 2^32 threads)
+// launch(items, how many of them are dq's): all in one grid, or where they are too many in one each.
+template <class F> int sequence_launch_both(int64_t dq_items, int64_t dkv_items, F launch) {
+  const bool both = dq_items + dkv_items <= kMostItems;
+  const int64_t first = both ? dq_items + dkv_items : dq_items, rest = both ? 0 : dkv_items;
+  if (first > 0) launch(first, dq_items);
+  XFH_TRY(check_launch("sequence_attention_backward"));
+  if (rest > 0) launch(rest, 0);
+  return check_launch("sequence_attention_backward");
+}
 // bf16 layouts that fit sequence_bf16_forward.hip and sequence_bf16_backward.hip, whose parts sequence.hip joins.
 bool sequence_bf16_forward_fits(const SequenceArgs &a);
 bool sequence_bf16_backward_fits(const SequenceArgs &a);

@@ -90,9 +90,9 @@ constexpr float kLowest = -3.402823466e38f;              // running maximum befo
 // D = 128, bf16: 72 us with the join, 79 with two equal parts each; of 5000 keys and three times 300: 51 and 78.
 struct Part {
   int b, blk, hk, index, count, slot;
-  __device__ __forceinline__ Part(const SequenceArgs &a, const Parts &parts, int blocks) {
-    hk = blockIdx.x % a.Hk;
-    int rest = blockIdx.x / a.Hk;
+  __device__ __forceinline__ Part(const SequenceArgs &a, const Parts &parts, int blocks, unsigned item) {
+    hk = int(item) % a.Hk;
+    int rest = int(item) / a.Hk;
     if (!parts.table) {
       index = rest % parts.splits;
       rest /= parts.splits;
@@ -164,10 +164,10 @@ struct Share { int head0, head1, tile0, tile1; };
 struct KeyItem {
   int b, hk, block, split;
   Share share;
-  __device__ __forceinline__ KeyItem(const SequenceArgs &a, const Splits &splits) {
+  __device__ __forceinline__ KeyItem(const SequenceArgs &a, const Splits &splits, unsigned item) {
     const int group = a.H / a.Hk, qtiles = (a.Nq + kTile - 1) / kTile, count = splits.heads * splits.tiles;
-    hk = blockIdx.x % a.Hk;
-    int rest = blockIdx.x / a.Hk;
+    hk = int(item) % a.Hk;
+    int rest = int(item) / a.Hk;
     b = rest % a.B;
     rest /= a.B;
     split = rest % count;

@@ -266,7 +266,7 @@ __global__ __launch_bounds__(256) void forward_kernel(SequenceArgs a, int blocks
   constexpr int P = DP + pitch_pad<T>();
   __shared__ __attribute__((aligned(16))) T ks[kTile * P], vs[kTile * P];
   __shared__ int ids[kTile];
-  const Part part(a, parts, blocks);
+  const Part part(a, parts, blocks, blockIdx.x);
   if (part.count == 0) return;
   const Columns own(a, part);
   const int b = own.b, h = own.h, hk = own.hk, i = own.i;
@@ -455,15 +455,28 @@ template <typename T, int N> __global__ __launch_bounds__(256) void join_kernel(
   if (a.lse && d == 0) put_stat<T>(a, row, top, sum);
 }
 
-// dq of 64 queries, their delta = dout . out (for dk and dv), and the slopes' part of each query,
+// delta = dout . out of each query, four lanes a row.
+template <typename T> __global__ __launch_bounds__(256) void delta_kernel(SequenceArgs a) {
+  const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> 2;
+  if (at >= int64_t(a.B) * a.H * a.Nq) return;           // (all lanes of a row)
+  const int i = int(at % a.Nq), h = int(at / a.Nq % a.H), b = int(at / a.Nq / a.H);
+  const T *gp = static_cast<const T *>(a.dout) + b * a.gs[0] + h * a.gs[1] + i * a.gs[2];
+  const T *op = static_cast<const T *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2];
+  const bf16 *low = a.low ? static_cast<const bf16 *>(a.low) + at * a.Dv : nullptr;
+  float delta = 0.f;
+  for (int d = threadIdx.x & 3; d < a.Dv; d += 4) delta += to_f32(gp[d]) * (to_f32(op[d]) + (low ? to_f32(low[d]) : 0.f));
+  delta += __shfl_xor(delta, 1, 64);
+  delta += __shfl_xor(delta, 2, 64);
+  if (threadIdx.x % 4 == 0) a.delta[at] = delta;
+}
+
+// dq of 64 queries, and the slopes' part of each query,
 //   - sum_j P (dP - sum P dP) |gap| = - (sum_j P (dP - delta) |gap| - (sum_j P (dP - delta)) (sum_j P |gap|)),
 // in fp32 from unrounded values: delta, which has the output's rounding in it, drops out, and so does
 // what the row's P are off by together, since each sum is divided by theirs.
-template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(SequenceArgs a, int blocks, bool vec) {
-  constexpr int P = DP + pitch_pad<T>();
-  __shared__ __attribute__((aligned(16))) T ks[kTile * P], vs[kTile * P];
-  __shared__ int ids[kTile];
-  const Columns own(a, Part(a, Parts{nullptr, nullptr, nullptr, 1, a.B}, blocks));
+template <typename T, int DP>
+__device__ __forceinline__ void dq_block(const SequenceArgs &a, int blocks, bool vec, unsigned item, T *ks, T *vs, int *ids) {
+  const Columns own(a, Part(a, Parts{nullptr, nullptr, nullptr, 1, a.B}, blocks, item));
   const int b = own.b, h = own.h, hk = own.hk, i = own.i;
   const int tid = threadIdx.x, lane = tid & 63, grp = lane >> 4;
   const Place &place = own.place;
@@ -474,17 +487,10 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
   typename Frag<T>::type qf[DP / 32], gf[DP / 32];
   load_own<T, DP>(qf, static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1] + i * a.qs[2], a.D, valid, grp, vec);
   const T *gp = static_cast<const T *>(a.dout) + b * a.gs[0] + h * a.gs[1] + i * a.gs[2];
-  const T *op = static_cast<const T *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2];
   load_own<T, DP>(gf, gp, a.Dv, valid, grp, vec);
-  float delta = 0.f;
   const int64_t at = (int64_t(b) * a.H + h) * a.Nq + i;
-  const bf16 *low = a.low ? static_cast<const bf16 *>(a.low) + at * a.Dv : nullptr;
-  if (valid)
-    for (int d0 = grp * 8; d0 < a.Dv; d0 += 32)
-      for (int d = d0; d < min(d0 + 8, a.Dv); ++d) delta += to_f32(gp[d]) * (to_f32(op[d]) + (low ? to_f32(low[d]) : 0.f));
-  delta = column_sum(delta);
+  const float delta = valid ? a.delta[at] : 0.f;
   const Stat stat = get_stat<T>(a, at, valid);
-  if (valid && grp == 0) a.delta[at] = delta;
   const auto test = [&](int tile) { return key_tile_needs(a, b, tile, own.span, own.span); };
   const Scorer<T> score(a, h);
 
@@ -571,13 +577,9 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void dq_kernel(S
 
 // dk and dv of 64 keys: over the heads that share them and the queries that see them (of a work item's share).
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void dkv_kernel(SequenceArgs a, Splits splits, float *parts, bool vec) {
-  constexpr int P = DP + pitch_pad<T>();
-  __shared__ __attribute__((aligned(16))) T qs[kTile * P], gs[kTile * P];
-  __shared__ Row rows[kTile];
-  __shared__ Stat stats[kTile];
-  __shared__ float deltas[kTile];
-  const KeyItem item(a, splits);
+__device__ __forceinline__ void dkv_block(const SequenceArgs &a, const Splits &splits, float *parts, bool vec, unsigned number,
+                                          T *qs, T *gs, Row *rows, Stat *stats, float *deltas) {
+  const KeyItem item(a, splits, number);
   const int hk = item.hk, b = item.b, block = item.block, group = a.H / a.Hk;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
   const Place place = place_of(a, b);
@@ -700,6 +702,22 @@ __global__ __launch_bounds__(256) void dkv_kernel(SequenceArgs a, Splits splits,
     }
 }
 
+// Both in one launch, dq's work items first, with dout . out from delta_kernel: each alone leaves CUs idle, at its end at
+// least. In fp32, one launch and two: 384 tokens in 3 chains, 16 heads of 24, 40 and 62 us; the backward pass of 2 x 1111, 8 heads on
+// 2, D = 64, 222 and 256 us; where there is work for all CUs 684 and 660 (2 x 1024, 16 heads of 96), 812 and 778 (4 x 2048, 8 of 32).
+// Up to 32 dims two workgroups fit a CU's registers, if the compiler is held to it (1161 us in the last case if not).
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP == 32 ? 2 : 1) void backward_kernel(SequenceArgs a, int blocks, int dq_items, Splits splits, float *parts, bool vec) {
+  constexpr int P = DP + pitch_pad<T>();
+  __shared__ __attribute__((aligned(16))) T tile0[kTile * P], tile1[kTile * P];
+  __shared__ Row rows[kTile];
+  __shared__ Stat stats[kTile];
+  __shared__ float deltas[kTile];
+  __shared__ int ids[kTile];
+  if (int(blockIdx.x) < dq_items) dq_block<T, DP>(a, blocks, vec, blockIdx.x, tile0, tile1, ids);
+  else dkv_block<T, DP>(a, splits, parts, vec, blockIdx.x - dq_items, tile0, tile1, rows, stats, deltas);
+}
+
 // dk and dv from the parts of their work items, in order: a thread per element, or per 4.
 template <typename T, int N> __global__ __launch_bounds__(256) void dkv_join_kernel(SequenceArgs a, int splits, const float *parts) {
   const int width = a.D + a.Dv, pieces = width / N;
@@ -757,18 +775,18 @@ template <typename T, int DP> int launch_forward(const SequenceArgs &a, const Pa
 template <typename T, int DP> int launch_backward(const SequenceArgs &a, const Splits &splits, float *parts, hipStream_t s) {
   const int64_t qblocks = ceil_div(int64_t(a.H / a.Hk) * a.Nq, int64_t(kTile)), kblocks = ceil_div(a.Nk, int64_t(kTile));
   const bool vec = vector_rows<T>({{a.k, a.ks}, {a.q, a.qs}}, a.D) && vector_rows<T>({{a.v, a.vs}, {a.dout, a.gs}}, a.Dv);
-  if (qblocks > 0) dq_kernel<T, DP><<<dim3(unsigned(qblocks * a.Hk * a.B)), 256, 0, s>>>(a, int(qblocks), vec);
+  const int64_t dq_items = qblocks * a.Hk * a.B, dkv_items = a.dk || a.dv ? kblocks * a.Hk * a.B * splits.heads * splits.tiles : 0;
+  if (dq_items > 0) delta_kernel<T><<<dim3(unsigned(ceil_div(int64_t(a.B) * a.H * a.Nq, int64_t(64)))), 256, 0, s>>>(a);
   XFH_TRY(check_launch("sequence_attention_backward"));
-  if (kblocks > 0 && (a.dk || a.dv))
-    dkv_kernel<T, DP><<<dim3(unsigned(kblocks * a.Hk * a.B * splits.heads * splits.tiles)), 256, 0, s>>>(a, splits, parts, vec);
-  return check_launch("sequence_attention_backward");
+  return sequence_launch_both(dq_items, dkv_items, [&](int64_t items, int64_t first) {
+    backward_kernel<T, DP><<<dim3(unsigned(items)), 256, 0, s>>>(a, int(qblocks), int(first), splits, parts, vec);
+  });
 }
 
 int check_grid(const SequenceArgs &a) {
   // At most 64 splits of a work item's keys, and those only of few work items.
   const int64_t most = std::max((ceil_div(int64_t(a.Nq), int64_t(kTile)) + 1) * a.H, ceil_div(int64_t(a.Nk), int64_t(kTile)) * a.Hk) * a.B;
-  // (A grid holds fewer than 2^32 threads.)
-  if (most > (int64_t(1) << 24) - 65536 || int64_t(a.H / std::max(a.Hk, 1)) * a.Nq > (int64_t(1) << 31) - 256)
+  if (most > kMostItems || int64_t(a.H / std::max(a.Hk, 1)) * a.Nq > (int64_t(1) << 31) - 256)
     return fail(XFH_EUNSUPPORTED, "sequence_attention: problem too large");
   return XFH_OK;
 }

@@ -1,4 +1,4 @@
-// Sequence attention in bf16 on 32x32x16 MFMAs (sequence_bf16.h), backward: dq, then dk and dv.
+// Sequence attention in bf16 on 32x32x16 MFMAs (sequence_bf16.h), backward: dq, dk and dv.
 //
 // dq: the columns are queries, as in the forward pass. dk and dv: the columns are 64 keys, the loop goes
 // over the heads of the group and their queries. Two kernels with 3 and 4 products, of which 2 are the same, in place of one with
@@ -100,13 +100,11 @@ __device__ __forceinline__ void dq_walk(const SequenceArgs &a, const Lane<D> &ln
   }
 }
 
-template <class D, int MODE>
-__global__ __launch_bounds__(256, 2) void dq_bf16_kernel(SequenceArgs a, int blocks) {
-  constexpr int TILE = kTile * D::DL;
-  __shared__ __attribute__((aligned(1024))) bf16 stage0[2 * TILE], stage1[2 * TILE];
-  __shared__ __attribute__((aligned(16))) Marks marks[4];
+// DELTA: dout . out is worked out here and kept for dk and dv; else it is there.
+template <class D, int MODE, bool DELTA>
+__device__ __forceinline__ void dq_block(const SequenceArgs &a, int blocks, int item, bf16 *stage0, bf16 *stage1, Marks *marks) {
   const int group = a.H / a.Hk, columns = group * a.Nq;
-  const int hk = blockIdx.x % a.Hk, rest = blockIdx.x / a.Hk, blk = blocks - 1 - rest % blocks, b = rest / blocks;
+  const int hk = item % a.Hk, rest = item / a.Hk, blk = blocks - 1 - rest % blocks, b = rest / blocks;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Lane<D> ln;
   const int c0 = blk * kColumns, c1 = min(c0 + kColumns, columns) - 1;
@@ -124,7 +122,7 @@ __global__ __launch_bounds__(256, 2) void dq_bf16_kernel(SequenceArgs a, int blo
   own_row<D>(gf, static_cast<const bf16 *>(a.dout) + b * a.gs[0] + h * a.gs[1] + i * a.gs[2], a.Dv, valid, ln.half);
   const int64_t at = (int64_t(b) * a.H + h) * a.Nq + i;
   float delta = 0.f;
-  {
+  if constexpr (DELTA) {
     bf16x8 of[D::KS], lf[D::KS] = {};
     own_row<D>(of, static_cast<const bf16 *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2], a.Dv, valid, ln.half);
     if (a.low) own_row<D>(lf, static_cast<const bf16 *>(a.low) + at * a.Dv, a.Dv, valid, ln.half);
@@ -133,10 +131,12 @@ __global__ __launch_bounds__(256, 2) void dq_bf16_kernel(SequenceArgs a, int blo
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         delta = __builtin_fmaf(static_cast<float>(of[ks][e]) + static_cast<float>(lf[ks][e]), static_cast<float>(gf[ks][e]), delta);
+    delta += other_half(delta);
+    if (valid && ln.half == 0) a.delta[at] = delta;
+  } else if (valid) {
+    delta = a.delta[at];
   }
-  delta += other_half(delta);
   const float lse = valid ? a.lse[at] : INFINITY;
-  if (valid && ln.half == 0) a.delta[at] = delta;
   const Loader<D, 4> kl(static_cast<const bf16 *>(a.k) + b * a.ks[0] + hk * a.ks[1], a.ks[2], place.n, a.D, wave);
   const Loader<D, 4> vl(static_cast<const bf16 *>(a.v) + b * a.vs[0] + hk * a.vs[1], a.vs[2], place.n, a.Dv, wave);
   const int end = (block.high + kTile - 1) / kTile;
@@ -340,14 +340,11 @@ __device__ __forceinline__ void dkv_walk(const SequenceArgs &a, const Lane<D> &l
 // Work item = (split, key block, batch entry, key head); the sums of split s go to parts [s][B Hk][Nk][D + Dv] in
 // fp32 when there are several.
 template <class D, int MODE>
-__global__ __launch_bounds__(256, 2) void dkv_bf16_kernel(SequenceArgs a, Splits splits, float *parts) {
-  constexpr int TILE = kTile * D::DL, T = D::DT / 2, STAGES = kDkvStages<D>;
+__device__ __forceinline__ void dkv_block(const SequenceArgs &a, const Splits &splits, float *parts, int at, bf16 *stage0,
+                                          bf16 *stage1, float *stats0, float *stats1, Exchange *exchange, Marks *marks) {
+  constexpr int T = D::DT / 2;
   static_assert(D::DT % 2 == 0, "two wavefronts share the head dim");
-  __shared__ __attribute__((aligned(1024))) bf16 stage0[2 * TILE], stage1[STAGES == 2 ? 2 * TILE : 8];
-  __shared__ __attribute__((aligned(1024))) float stats0[2 * kTile], stats1[STAGES == 2 ? 2 * kTile : 4];
-  __shared__ __attribute__((aligned(16))) Exchange exchange[4];
-  __shared__ __attribute__((aligned(16))) Marks marks[4];
-  const KeyItem item(a, splits);
+  const KeyItem item(a, splits, at);
   const int hk = item.hk, b = item.b;
   const Share &share = item.share;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave >> 1;
@@ -392,6 +389,65 @@ __global__ __launch_bounds__(256, 2) void dkv_bf16_kernel(SequenceArgs a, Splits
   store_column(static_cast<bf16 *>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2] + d0, a.Dv - d0, dv, 1.f, ln.half);
 }
 
+// ------------------------------------------------------------------------------ launches
+
+template <class D, int MODE> __global__ __launch_bounds__(256, 2) void dq_bf16_kernel(SequenceArgs a, int blocks) {
+  constexpr int TILE = kTile * D::DL;
+  __shared__ __attribute__((aligned(1024))) bf16 stage0[2 * TILE], stage1[2 * TILE];
+  __shared__ __attribute__((aligned(16))) Marks marks[4];
+  dq_block<D, MODE, true>(a, blocks, blockIdx.x, stage0, stage1, marks);
+}
+
+template <class D, int MODE>
+__global__ __launch_bounds__(256, 2) void dkv_bf16_kernel(SequenceArgs a, Splits splits, float *parts) {
+  constexpr int TILE = kTile * D::DL, STAGES = kDkvStages<D>;
+  __shared__ __attribute__((aligned(1024))) bf16 stage0[2 * TILE], stage1[STAGES == 2 ? 2 * TILE : 8];
+  __shared__ __attribute__((aligned(1024))) float stats0[2 * kTile], stats1[STAGES == 2 ? 2 * kTile : 4];
+  __shared__ __attribute__((aligned(16))) Exchange exchange[4];
+  __shared__ __attribute__((aligned(16))) Marks marks[4];
+  dkv_block<D, MODE>(a, splits, parts, blockIdx.x, stage0, stage1, stats0, stats1, exchange, marks);
+}
+
+// Both in one launch, dq's work items first, with dout . out from delta_bf16_kernel (3 us): each alone leaves CUs idle at
+// its end, and with few work items all along. Forward and backward of 3 x 1111 tokens, 8 heads on 2, D = 64: 116 us in two
+// launches, 97 in one; 5 x 768, 16 heads of 48, with slopes: 163 and 154; the backward pass of 2 x 2048, 16 heads on 4, D = 64: 154
+// and 128, of 4 x 4096 1359 in both. Head dims over 64 stay in two: with the stages of both a CU would hold one workgroup.
+template <class E> constexpr bool kOneLaunch = kDkvStages<E> == 2;
+template <class D, class E, int MODE>
+__global__ __launch_bounds__(256, 2) void backward_bf16_kernel(SequenceArgs a, int blocks, int dq_items, Splits splits, float *parts) {
+  static_assert(D::DL <= E::DL, "dq takes the stages of dk and dv");
+  constexpr int TILE = kTile * E::DL;
+  __shared__ __attribute__((aligned(1024))) bf16 stage0[2 * TILE], stage1[2 * TILE];
+  __shared__ __attribute__((aligned(1024))) float stats0[2 * kTile], stats1[2 * kTile];
+  __shared__ __attribute__((aligned(16))) Exchange exchange[4];
+  __shared__ __attribute__((aligned(16))) Marks marks[4];
+  const int item = blockIdx.x;
+  if (item < dq_items) dq_block<D, MODE, false>(a, blocks, item, stage0, stage1, marks);
+  else dkv_block<E, MODE>(a, splits, parts, item - dq_items, stage0, stage1, stats0, stats1, exchange, marks);
+}
+
+// delta[row] = dout . out, two lanes a row: summed in the order that dq_block has it in.
+__global__ __launch_bounds__(256) void delta_bf16_kernel(SequenceArgs a) {
+  const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> 1;
+  if (at >= int64_t(a.B) * a.H * a.Nq) return;           // (both lanes of a row)
+  const int i = int(at % a.Nq), h = int(at / a.Nq % a.H), b = int(at / a.Nq / a.H);
+  const bf16 *o = static_cast<const bf16 *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2];
+  const bf16 *g = static_cast<const bf16 *>(a.dout) + b * a.gs[0] + h * a.gs[1] + i * a.gs[2];
+  const bf16 *low = a.low ? static_cast<const bf16 *>(a.low) + at * a.Dv : nullptr;
+  float delta = 0.f;
+#pragma unroll 4
+  for (int d = (threadIdx.x & 1) * 8; d < a.Dv; d += 16) {
+    const bf16x8 of = *reinterpret_cast<const bf16x8 *>(o + d), gf = *reinterpret_cast<const bf16x8 *>(g + d);
+    bf16x8 lf = {};
+    if (low) lf = *reinterpret_cast<const bf16x8 *>(low + d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      delta = __builtin_fmaf(static_cast<float>(of[e]) + static_cast<float>(lf[e]), static_cast<float>(gf[e]), delta);
+  }
+  delta += __shfl_xor(delta, 1, 64);
+  if (threadIdx.x % 2 == 0) a.delta[at] = delta;
+}
+
 }  // namespace
 
 bool sequence_bf16_backward_fits(const SequenceArgs &a) {
@@ -406,10 +462,18 @@ int sequence_bf16_backward(const SequenceArgs &a, const Splits &splits, float *p
     typedef decltype(dim) D;
     typedef Dim<D::DL < 64 ? 64 : D::DL, D::KS, D::DT + D::DT % 2> E;    // (two wavefronts share the head dim)
     constexpr int MODE = decltype(mode)::value;
-    if (blocks > 0) dq_bf16_kernel<D, MODE><<<dim3(unsigned(blocks * a.Hk * a.B)), 256, 0, s>>>(a, int(blocks));
-    XFH_TRY(check_launch("sequence_attention_backward"));
-    if (kblocks > 0 && (a.dk || a.dv))
-      dkv_bf16_kernel<E, MODE><<<dim3(unsigned(kblocks * a.Hk * a.B * splits.heads * splits.tiles)), 256, 0, s>>>(a, splits, parts);
+    const int64_t dq_items = blocks * a.Hk * a.B, dkv_items = a.dk || a.dv ? kblocks * a.Hk * a.B * splits.heads * splits.tiles : 0;
+    if constexpr (kOneLaunch<E>) {
+      if (dq_items > 0) delta_bf16_kernel<<<dim3(unsigned(ceil_div(int64_t(a.B) * a.H * a.Nq, int64_t(128)))), 256, 0, s>>>(a);
+      XFH_TRY(check_launch("sequence_attention_backward"));
+      return sequence_launch_both(dq_items, dkv_items, [&](int64_t items, int64_t first) {
+        backward_bf16_kernel<D, E, MODE><<<dim3(unsigned(items)), 256, 0, s>>>(a, int(blocks), int(first), splits, parts);
+      });
+    } else {
+      if (dq_items > 0) dq_bf16_kernel<D, MODE><<<dim3(unsigned(dq_items)), 256, 0, s>>>(a, int(blocks));
+      XFH_TRY(check_launch("sequence_attention_backward"));
+      if (dkv_items > 0) dkv_bf16_kernel<E, MODE><<<dim3(unsigned(dkv_items)), 256, 0, s>>>(a, splits, parts);
+    }
     return check_launch("sequence_attention_backward");
   });
 }

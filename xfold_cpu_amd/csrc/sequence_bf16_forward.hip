@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256, 2) void forward_bf16_kernel(SequenceArgs a, in
   __shared__ __attribute__((aligned(1024))) bf16 stage0[2 * TILE], stage1[2 * TILE];
   __shared__ __attribute__((aligned(16))) Marks marks[4];
   const int group = a.H / a.Hk, columns = group * a.Nq;
-  const Part part(a, parts, blocks);
+  const Part part(a, parts, blocks, blockIdx.x);
   if (part.count == 0) return;
   const int b = part.b, hk = part.hk, blk = part.blk;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256, 1) void token_bf16_kernel(SequenceArgs a, Part
   static_assert(sizeof(stage0) >= 2 * 32 * PITCH * 4, "two wavefronts' results are joined in a stage");
   const auto joined = [&](int w) { return reinterpret_cast<float *>(w < 2 ? stage0 : stage1) + (w & 1) * 32 * PITCH; };
   const int group = a.H / a.Hk, columns = group * a.Nq;
-  const Part part(a, parts, 1);
+  const Part part(a, parts, 1, blockIdx.x);
   const int b = part.b, hk = part.hk;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Lane<D> ln;
