@@ -65,11 +65,19 @@ __device__ __forceinline__ void dq_walk(const SequenceArgs &a, const Lane<D> &ln
         }
         w[r] = Score<MODE>::CAP ? ds * bent[r] : ds;
       }
+      // dS in two bf16 pieces: in one, its rounding (relative rms 2^-9, no less than the output's own, and more where
+      // the sum over the keys cancels) is most of dq's error: 2.4e-3 to 2.9e-3 of its norm, 1.7e-3 to 2.2e-3 in two. With
+      // slopes 5 x 768 tokens take 158 us in place of 154, long runs 4 x 4096 1508 in place of 1350. At D = 128
+      // there are no registers for it (error 2.4e-3 to 2.6e-3).
+      f32x16 rest;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rest[r] = w[r] - static_cast<float>(bf16(w[r]));
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         bf16x8 tf[D::DT];
         ln.transposed_fragments(kt, 2 * rt + s, tf);
         add_product<STRICT, false>(tf, weights(w, 8 * s), weights_seen(seen, 8 * s), dq);
+        if constexpr (D::DL <= 64) add_product<STRICT, false>(tf, weights(rest, 8 * s), bf16x8{}, dq);
       }
     }
   };
@@ -411,7 +419,7 @@ __global__ __launch_bounds__(256, 2) void dkv_bf16_kernel(SequenceArgs a, Splits
 // Both in one launch, dq's work items first, with dout . out from delta_bf16_kernel (3 us): each alone leaves CUs idle at
 // its end, and with few work items all along. Forward and backward of 3 x 1111 tokens, 8 heads on 2, D = 64: 116 us in two
 // launches, 97 in one; 5 x 768, 16 heads of 48, with slopes: 163 and 154; the backward pass of 2 x 2048, 16 heads on 4, D = 64: 154
-// and 128, of 4 x 4096 1359 in both. Head dims over 64 stay in two: with the stages of both a CU would hold one workgroup.
+// and 128, of 4 x 4096 1359 in both (before dS was in two pieces). Head dims over 64 stay in two: with the stages of both a CU would hold one workgroup.
 template <class E> constexpr bool kOneLaunch = kDkvStages<E> == 2;
 template <class D, class E, int MODE>
 __global__ __launch_bounds__(256, 2) void backward_bf16_kernel(SequenceArgs a, int blocks, int dq_items, Splits splits, float *parts) {
