@@ -416,11 +416,12 @@ __global__ __launch_bounds__(256, 2) void dkv_bf16_kernel(SequenceArgs a, Splits
   dkv_block<D, MODE>(a, splits, parts, blockIdx.x, stage0, stage1, stats0, stats1, exchange, marks);
 }
 
-// Both in one launch, dq's work items first, with dout . out from delta_bf16_kernel (3 us): each alone leaves CUs idle at
+// Both in one launch, dq's work items first, with dout . out from delta_bf16_kernel (6 us at 5 x 768 tokens of 16 heads of 48): each alone leaves CUs idle at
 // its end, and with few work items all along. Forward and backward of 3 x 1111 tokens, 8 heads on 2, D = 64: 116 us in two
 // launches, 97 in one; 5 x 768, 16 heads of 48, with slopes: 163 and 154; the backward pass of 2 x 2048, 16 heads on 4, D = 64: 154
 // and 128, of 4 x 4096 1359 in both (before dS was in two pieces). Head dims over 64 stay in two: with the stages of both a CU would hold one workgroup.
 template <class E> constexpr bool kOneLaunch = kDkvStages<E> == 2;
+static_assert(kOneLaunch<Dim<64, 4, 2>> && !kOneLaunch<Dim<128, 8, 4>>, "delta_bf16_kernel takes up to 64 dims");
 template <class D, class E, int MODE>
 __global__ __launch_bounds__(256, 2) void backward_bf16_kernel(SequenceArgs a, int blocks, int dq_items, Splits splits, float *parts) {
   static_assert(D::DL <= E::DL, "dq takes the stages of dk and dv");
@@ -434,26 +435,24 @@ __global__ __launch_bounds__(256, 2) void backward_bf16_kernel(SequenceArgs a, i
   else dkv_block<E, MODE>(a, splits, parts, item - dq_items, stage0, stage1, stats0, stats1, exchange, marks);
 }
 
-// delta[row] = dout . out, two lanes a row: summed in the order that dq_block has it in.
+// delta[row] = dout . out of up to 64 dims: eight lanes a row, 16 bytes each.
 __global__ __launch_bounds__(256) void delta_bf16_kernel(SequenceArgs a) {
-  const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> 1;
-  if (at >= int64_t(a.B) * a.H * a.Nq) return;           // (both lanes of a row)
-  const int i = int(at % a.Nq), h = int(at / a.Nq % a.H), b = int(at / a.Nq / a.H);
-  const bf16 *o = static_cast<const bf16 *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2];
-  const bf16 *g = static_cast<const bf16 *>(a.dout) + b * a.gs[0] + h * a.gs[1] + i * a.gs[2];
-  const bf16 *low = a.low ? static_cast<const bf16 *>(a.low) + at * a.Dv : nullptr;
-  float delta = 0.f;
-#pragma unroll 4
-  for (int d = (threadIdx.x & 1) * 8; d < a.Dv; d += 16) {
-    const bf16x8 of = *reinterpret_cast<const bf16x8 *>(o + d), gf = *reinterpret_cast<const bf16x8 *>(g + d);
-    bf16x8 lf = {};
-    if (low) lf = *reinterpret_cast<const bf16x8 *>(low + d);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      delta = __builtin_fmaf(static_cast<float>(of[e]) + static_cast<float>(lf[e]), static_cast<float>(gf[e]), delta);
+  const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> 3;
+  if (at >= int64_t(a.B) * a.H * a.Nq) return;           // (all lanes of a row)
+  const int i = int(at % a.Nq), h = int(at / a.Nq % a.H), b = int(at / a.Nq / a.H), d = (threadIdx.x & 7) * 8;
+  bf16x8 of = {}, gf = {}, lf = {};
+  if (d < a.Dv) {
+    of = *reinterpret_cast<const bf16x8 *>(static_cast<const bf16 *>(a.out) + b * a.os[0] + h * a.os[1] + i * a.os[2] + d);
+    gf = *reinterpret_cast<const bf16x8 *>(static_cast<const bf16 *>(a.dout) + b * a.gs[0] + h * a.gs[1] + i * a.gs[2] + d);
+    if (a.low) lf = *reinterpret_cast<const bf16x8 *>(static_cast<const bf16 *>(a.low) + at * a.Dv + d);
   }
-  delta += __shfl_xor(delta, 1, 64);
-  if (threadIdx.x % 2 == 0) a.delta[at] = delta;
+  float delta = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    delta = __builtin_fmaf(static_cast<float>(of[e]) + static_cast<float>(lf[e]), static_cast<float>(gf[e]), delta);
+#pragma unroll
+  for (int o = 1; o < 8; o *= 2) delta += __shfl_xor(delta, o, 64);
+  if (threadIdx.x % 8 == 0) a.delta[at] = delta;
 }
 
 }  // namespace
@@ -472,7 +471,7 @@ int sequence_bf16_backward(const SequenceArgs &a, const Splits &splits, float *p
     constexpr int MODE = decltype(mode)::value;
     const int64_t dq_items = blocks * a.Hk * a.B, dkv_items = a.dk || a.dv ? kblocks * a.Hk * a.B * splits.heads * splits.tiles : 0;
     if constexpr (kOneLaunch<E>) {
-      if (dq_items > 0) delta_bf16_kernel<<<dim3(unsigned(ceil_div(int64_t(a.B) * a.H * a.Nq, int64_t(128)))), 256, 0, s>>>(a);
+      if (dq_items > 0) delta_bf16_kernel<<<dim3(unsigned(ceil_div(int64_t(a.B) * a.H * a.Nq, int64_t(32)))), 256, 0, s>>>(a);
       XFH_TRY(check_launch("sequence_attention_backward"));
       return sequence_launch_both(dq_items, dkv_items, [&](int64_t items, int64_t first) {
         backward_bf16_kernel<D, E, MODE><<<dim3(unsigned(items)), 256, 0, s>>>(a, int(blocks), int(first), splits, parts);
