@@ -452,3 +452,16 @@ def test_captured_call_reads_the_lengths_of_its_replay(device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, call()), now
+
+
+def test_refusals_of_the_library_are_value_errors(device):
+    from xfold_cpu_amd import fastnn
+    from xfold_cpu_amd.fastnn import native_hip as nh
+    q, k, v, _ = data(device, F32, 1, 1, 1, 5, 5, 4)
+    for leaf in (q, q.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="softcap too small"):
+            fastnn.sequence_attention(leaf, k, v, softcap=1e-39)
+        with pytest.raises(ValueError, match="eps must be nonnegative"):
+            nh.autograd().trainable_layer_norm(leaf, None, None, 4, -1.0, False)
+    out = fastnn.sequence_attention(q, k, v)                       # nothing is left behind
+    assert torch.equal(out, fastnn.sequence_attention(q, k, v))

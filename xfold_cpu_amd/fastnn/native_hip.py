@@ -106,10 +106,6 @@ SIGNATURES = {
 }
 
 
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
 class HipBackendError(RuntimeError):
     """A libxfold_hip call returned an error status."""
 
@@ -183,16 +179,6 @@ def autograd():
     loader.exec_module(module)
     module.bind(ABI_VERSION, {name: ctypes.cast(function(name), ctypes.c_void_p).value for name in SIGNATURES})
     return module
-
-
-def launch(device: torch.device, name: str, *args) -> None:
-    """:func:`call` with ``device`` as the current one and its current stream as the last argument."""
-    index = device.index
-    if index != _current_device():
-        with torch.cuda.device(index):
-            return call(name, *args, _raw_stream(index))
-    if function(name)(*args, _raw_stream(index)) != 0:
-        call(name, *args, _raw_stream(index))            # (again, for the error: what failed launched nothing)
 
 
 def set_kernel_timing(enable: bool) -> None:
